@@ -56,6 +56,13 @@ extern "C" {
 #define STACR_MODE_CHUNK_TOPK 0
 #define STACR_MODE_GLOBAL_TOPK 1
 
+/* activations of the gated feed-forward block */
+#define STACR_ACT_SILU 0      /* g / (1 + exp(-g)) */
+#define STACR_ACT_GELU 1      /* g (1 + erf(g / sqrt 2)) / 2 */
+#define STACR_ACT_GELU_TANH 2 /* g (1 + tanh(sqrt(2 / pi) (g + 0.044715 g^3))) / 2 */
+#define STACR_ACT_RELU 3      /* max(g, 0), slope 0 at 0 */
+#define STACR_ACT_SIGMOID 4   /* 1 / (1 + exp(-g)) */
+
 /* status codes */
 #define STACR_OK 0
 #define STACR_ERR_INVALID 1     /* bad argument (shape, dtype, null pointer, size) */
@@ -484,6 +491,37 @@ int stacr_qr(const float *a, int64_t rows, int cols, float *q, float *r, void *s
 int stacr_qr_tall_workspace_bytes(int64_t rows, int cols, size_t *bytes);
 int stacr_qr_tall(const float *a, int64_t rows, int cols, float *q, float *r, void *workspace,
                   size_t workspace_bytes, void *stream);
+
+/*
+ * Gated feed-forward block (no counterpart in the reference, whose layers wrap its projections):
+ *   g = x Wg^T + bg, u = x Wu^T + bu, h = act(g) * u
+ * x: rows x d with rows x_ld >= d values apart; w_gate, w_up: ff x d (row-major, as nn.Linear keeps
+ * them); biases ff values or NULL; h (and gate, up: g and u rounded, both or neither): rows x ff.  One
+ * type throughout; sums in fp32 (fp32 inputs: to fp32 accuracy).  The workspace holds operands whose
+ * rows are not whole, aligned groups of 8 values in another form (fp32: always), so its size depends on
+ * the pointers' alignment, which is all that the query looks at.  rows 0 is a no-op.  d, ff and x_ld at
+ * most 2^20, rows below 2^24 (STACR_ERR_UNSUPPORTED).
+ */
+int stacr_gated_workspace_bytes(const void *x, int dtype, int64_t rows, int64_t d, int64_t x_ld, const void *w_gate,
+                                const void *w_up, int64_t ff, int backward, size_t *bytes);
+int stacr_gated_forward(const void *x, int dtype, int64_t rows, int64_t d, int64_t x_ld, const void *w_gate,
+                        const void *w_up, int64_t ff, const void *b_gate, const void *b_up, int activation, void *h,
+                        void *gate, void *up, void *workspace, size_t workspace_bytes, void *stream);
+/*
+ * Its gradients for dh (rows x ff): dg = dh u act'(g), du = dh act(g), dx = dg Wg + du Wu (rows x d),
+ * dW_gate = dg^T x, dW_up = du^T x (ff x d), db = column sums.  gate and up as the forward kept them, or
+ * both NULL: g and u are then computed again from x and the weights, so that a caller keeps nothing but x.
+ * Each of dx, (dw_gate, dw_up), db_gate, db_up may be NULL.  x may be NULL when gate and up are given and
+ * no weight gradient is asked for; the weights may be when dx is not either.  dg and du are rounded to
+ * the type before the products.  dgu (16-bit types; NULL: kept in the workspace) receives [dg | du], rows
+ * x 2 p with p = ff rounded up to 8 and zeros past ff: the gradient that a weight-gradient call on x's
+ * saved factors takes for both projections at once.
+ */
+int stacr_gated_backward(const void *dh, const void *x, int dtype, int64_t rows, int64_t d, int64_t x_ld,
+                         const void *w_gate, const void *w_up, int64_t ff, const void *b_gate, const void *b_up,
+                         int activation, const void *gate, const void *up, void *dx, void *dw_gate, void *dw_up,
+                         void *db_gate, void *db_up, void *dgu, void *workspace, size_t workspace_bytes,
+                         void *stream);
 
 /*
  * Kernel timing (benchmarking aid; no counterpart in the reference).  Between begin and end,

@@ -6,6 +6,7 @@ include/stacr_amd.h); this package is the host side.
 """
 from .adaptive import AdaptiveSTACRConfig, AdaptiveSTACRLinear, apply_adaptive_stacr, set_stacr_runtime_state
 from .compressor import STACRCompressor, STACRConfig, stacr_saved_tensors
+from .gated import gated_feed_forward
 from .layers import STACRFunction, STACRLinear
 from .memory import saved_surface_predictor, stacr_stored_bytes
 from .quant import QuantizedValues, quantize_values
@@ -29,4 +30,5 @@ __all__ = [
     "AdaptiveSTACRLinear",
     "apply_adaptive_stacr",
     "set_stacr_runtime_state",
+    "gated_feed_forward",
 ]

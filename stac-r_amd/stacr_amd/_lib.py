@@ -22,6 +22,7 @@ STACR_ERR_HIP = 4
 DTYPE_F32, DTYPE_BF16, DTYPE_F16 = 0, 1, 2
 MODE_CHUNK_TOPK, MODE_GLOBAL_TOPK = 0, 1
 MAX_RANK = 32
+ACTIVATION_CODES = {"silu": 0, "gelu": 1, "gelu_tanh": 2, "relu": 3, "sigmoid": 4}
 SCALE_F64 = 3  # scale record dtype code: fp64 (an fp32 scale that underflowed)
 
 # Every symbol declared in include/stacr_amd.h, with its ctypes signature.
@@ -90,6 +91,10 @@ SIGNATURES = {
     "stacr_c1_workspace_bytes": ([_i64, _i64, _i32, _p], _i32),
     "stacr_c1_observe": ([_p, _i32, _i64, _i64, _p, _p, _i32, _i32, _p, _p, _p, _sz, _p], _i32),
     "stacr_c1_store": ([_p, _i64, _i32, _p, _i32, _p, _i32, _p], _i32),
+    "stacr_gated_workspace_bytes": ([_p, _i32, _i64, _i64, _i64, _p, _p, _i64, _i32, _PSZ], _i32),
+    "stacr_gated_forward": ([_p, _i32, _i64, _i64, _i64, _p, _p, _i64, _p, _p, _i32, _p, _p, _p, _p, _sz, _p], _i32),
+    "stacr_gated_backward": ([_p, _p, _i32, _i64, _i64, _i64, _p, _p, _i64, _p, _p, _i32, _p, _p, _p, _p, _p, _p, _p,
+                              _p, _p, _sz, _p], _i32),
     "stacr_c1_restore": ([_p, _i32, _p, _p, _i32, _i64, _i64, _i32, _p, _i32, _p], _i32),
 }
 

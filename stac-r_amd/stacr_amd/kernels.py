@@ -563,3 +563,72 @@ def c1_restore(coeff: torch.Tensor, scales: torch.Tensor | None, basis: torch.Te
                                   _ptr(basis), dtype_code(basis.dtype), rows, hidden, rank, _ptr(out), dtype_code(dtype),
                                   _stream(coeff.device)), "stacr_c1_restore")
     return out
+
+
+# ------------------------------------------------------------------ gated feed-forward block
+def _gated_workspace(x2d, dtype, rows, d, x_ld, w_gate, w_up, backward):
+    nbytes = ctypes.c_size_t()
+    _lib.check(_lib.load().stacr_gated_workspace_bytes(_ptr(x2d), dtype_code(dtype), rows, d, x_ld, _ptr(w_gate),
+                                                       _ptr(w_up), w_gate.shape[0], int(backward),
+                                                       ctypes.byref(nbytes)), "stacr_gated_workspace_bytes")
+    if not nbytes.value:
+        return None, 0
+    return torch.empty(nbytes.value, dtype=torch.uint8, device=w_gate.device), nbytes.value
+
+
+def _rows_of(x2d):
+    """A matrix whose rows are contiguous (any row stride of at least the row's length, up to the library's limit); a single row's
+    stride, which means nothing, is its length."""
+    rows, d = x2d.shape
+    if x2d.stride(1) == 1 or d == 1:
+        if d <= x2d.stride(0) <= 1 << 20 and rows > 1:
+            return x2d
+        if rows <= 1:
+            return x2d.as_strided((rows, d), (d, 1))
+    return x2d.contiguous()
+
+
+def gated_forward(x2d: torch.Tensor, w_gate: torch.Tensor, w_up: torch.Tensor, b_gate: torch.Tensor | None = None,
+                  b_up: torch.Tensor | None = None, activation: str = "silu", keep: bool = False):
+    """h = act(x Wg^T + bg) * (x Wu^T + bu) of rows x d (stacr_gated_forward); with ``keep`` (h, g, u), the
+    pre-activations rounded to the type.  The caller has checked shapes, types and devices
+    (gated.gated_feed_forward does)."""
+    x2d, w_gate, w_up = _rows_of(x2d), w_gate.contiguous(), w_up.contiguous()
+    rows, d = x2d.shape
+    ff = w_gate.shape[0]
+    h = torch.empty(rows, ff, dtype=x2d.dtype, device=x2d.device)
+    gate, up = (torch.empty_like(h), torch.empty_like(h)) if keep else (None, None)
+    ws, nbytes = _gated_workspace(x2d, x2d.dtype, rows, d, x2d.stride(0), w_gate, w_up, False)
+    _lib.check(_lib.load().stacr_gated_forward(_ptr(x2d), dtype_code(x2d.dtype), rows, d, x2d.stride(0), _ptr(w_gate),
+                                               _ptr(w_up), ff, _ptr(b_gate), _ptr(b_up),
+                                               _lib.ACTIVATION_CODES[activation], _ptr(h), _ptr(gate), _ptr(up),
+                                               _ptr(ws), nbytes, _stream(x2d.device)), "stacr_gated_forward")
+    return (h, gate, up) if keep else h
+
+
+def gated_backward(dh: torch.Tensor, x2d: torch.Tensor | None, w_gate: torch.Tensor, w_up: torch.Tensor,
+                   b_gate: torch.Tensor | None = None, b_up: torch.Tensor | None = None, activation: str = "silu",
+                   kept=None, needs=(True, True, False, False), slopes: bool = False):
+    """(dx, dw_gate, dw_up, db_gate, db_up, dgu) for dh, None where ``needs`` (input, weights, gate bias, up
+    bias) asks for none (stacr_gated_backward).  ``kept``: (g, u) of the forward, or None to compute them
+    again from x2d, which may be None with them when no weight gradient is asked for.  ``slopes``: give
+    out dgu = [dg | du], rows x 2 p with p = ff rounded up to 8 (16-bit types)."""
+    dh, w_gate, w_up = dh.contiguous(), w_gate.contiguous(), w_up.contiguous()
+    rows, ff = dh.shape
+    d, dtype, dev = w_gate.shape[1], dh.dtype, dh.device
+    if x2d is not None:
+        x2d = _rows_of(x2d)
+    dx = torch.empty(rows, d, dtype=dtype, device=dev) if needs[0] else None
+    dwg, dwu = (torch.empty_like(w_gate), torch.empty_like(w_up)) if needs[1] else (None, None)
+    dbg = torch.empty(ff, dtype=dtype, device=dev) if needs[2] else None
+    dbu = torch.empty(ff, dtype=dtype, device=dev) if needs[3] else None
+    dgu = torch.empty(rows, 2 * ((ff + 7) // 8 * 8), dtype=dtype, device=dev) if slopes else None
+    gate, up = kept if kept is not None else (None, None)
+    x_ld = x2d.stride(0) if x2d is not None else d
+    ws, nbytes = _gated_workspace(x2d, dtype, rows, d, x_ld, w_gate, w_up, True)
+    _lib.check(_lib.load().stacr_gated_backward(_ptr(dh), _ptr(x2d), dtype_code(dtype), rows, d, x_ld, _ptr(w_gate),
+                                                _ptr(w_up), ff, _ptr(b_gate), _ptr(b_up),
+                                                _lib.ACTIVATION_CODES[activation], _ptr(gate), _ptr(up), _ptr(dx),
+                                                _ptr(dwg), _ptr(dwu), _ptr(dbg), _ptr(dbu), _ptr(dgu), _ptr(ws),
+                                                nbytes, _stream(dev)), "stacr_gated_backward")
+    return dx, dwg, dwu, dbg, dbu, dgu
