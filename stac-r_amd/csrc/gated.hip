@@ -16,6 +16,8 @@
 // |a| |b|, where fp32's own rounding of the sum is 2^-24 a step.  A fourth plane holds hi with
 // infinities and NaN replaced by 0, which the five smaller products take, so that a non-finite value
 // meets the other operand once, in hi * hi, as it would in fp32.
+#include <type_traits>
+
 #include "matmul_tile.h"
 
 using namespace stacr;
@@ -40,7 +42,7 @@ struct MmArgs {
     void *out, *out2;
     int64_t ldo;
     int out_dt;
-    bool vec;                        // rows of out take aligned stores of four
+    bool vec;                        // rows of out (and dh) are whole, aligned 16-byte pieces
     float *part;                     // splits > 1: fp32 partial products [split][half][M][N]
     // gated epilogues
     const void *bias_g, *bias_u, *dh;
@@ -51,51 +53,64 @@ struct MmArgs {
 };
 
 // ------------------------------------------------------------------ activations
-// fp32 takes the accurate library functions, the 16-bit types v_exp_f32's (about 1e-6 relative at
-// |x| < 20, a thousandth of their rounding).
+// fp32 takes the accurate library functions and divisions, the 16-bit types the exponential and the
+// reciprocal of one instruction (about 1e-6 relative at |x| < 20, a thousandth of their rounding).
 template <bool EXACT> __device__ __forceinline__ float exp_of(float x)
 {
     if constexpr (EXACT) return expf(x);
     else return __expf(x);
 }
 
-// act(g) and act'(g)
-template <bool EXACT> __device__ __forceinline__ void activate(int act, float g, float &a, float &slope)
+template <bool EXACT> __device__ __forceinline__ float inverse(float x)
 {
-    switch (act) {
-    case STACR_ACT_SILU: {
-        const float s = 1.0f / (1.0f + exp_of<EXACT>(-g));
+    if constexpr (EXACT) return 1.0f / x;
+    else return __builtin_amdgcn_rcpf(x);
+}
+
+// act(g) and act'(g)
+template <bool EXACT, int ACT> __device__ __forceinline__ void activate(float g, float &a, float &slope)
+{
+    if constexpr (ACT == STACR_ACT_SILU) {
+        const float s = inverse<EXACT>(1.0f + exp_of<EXACT>(-g));
         a = g * s;
         slope = s * (1.0f + g * (1.0f - s));
-        break;
-    }
-    case STACR_ACT_GELU: {
+    } else if constexpr (ACT == STACR_ACT_GELU) {
         const float below = 0.5f * (1.0f + erff(g * 0.70710678118654752f));
         a = g * below;
         slope = below + g * 0.39894228040143268f * exp_of<EXACT>(-0.5f * g * g);
-        break;
-    }
-    case STACR_ACT_GELU_TANH: {
+    } else if constexpr (ACT == STACR_ACT_GELU_TANH) {
         const float in = 0.79788456080286536f * (g + 0.044715f * g * g * g);
-        const float t = 1.0f - 2.0f / (1.0f + exp_of<EXACT>(2.0f * in));
+        const float t = 1.0f - 2.0f * inverse<EXACT>(1.0f + exp_of<EXACT>(2.0f * in));
         a = 0.5f * g * (1.0f + t);
         slope = 0.5f * (1.0f + t) +
                 0.5f * g * (1.0f - t * t) * 0.79788456080286536f * (1.0f + 3.0f * 0.044715f * g * g);
-        break;
-    }
-    case STACR_ACT_RELU:
+    } else if constexpr (ACT == STACR_ACT_RELU) {
         a = g > 0.0f ? g : (g != g ? g : 0.0f);
         slope = g > 0.0f ? 1.0f : 0.0f;
-        break;
-    default: {
-        const float s = 1.0f / (1.0f + exp_of<EXACT>(-g));
+    } else {
+        const float s = inverse<EXACT>(1.0f + exp_of<EXACT>(-g));
         a = s;
         slope = s * (1.0f - s);
     }
+}
+
+// f(the activation's code as a constant): the choice is made once, outside the unrolled epilogues, whose
+// code would not fit the instruction cache with a choice a value
+template <typename F> __device__ __forceinline__ void with_activation(int act, F &&f)
+{
+    switch (act) {
+    case STACR_ACT_SILU: f(std::integral_constant<int, STACR_ACT_SILU>()); break;
+    case STACR_ACT_GELU: f(std::integral_constant<int, STACR_ACT_GELU>()); break;
+    case STACR_ACT_GELU_TANH: f(std::integral_constant<int, STACR_ACT_GELU_TANH>()); break;
+    case STACR_ACT_RELU: f(std::integral_constant<int, STACR_ACT_RELU>()); break;
+    default: f(std::integral_constant<int, STACR_ACT_SIGMOID>());
     }
 }
 
-__device__ __forceinline__ uint32_t pack_bf16(float lo, float hi) { return f_to_bf16_bits(lo) | f_to_bf16_bits(hi) << 16; }
+template <bool EXACT> __device__ __forceinline__ void activate(int act, float g, float &a, float &slope)
+{
+    with_activation(act, [&](auto c) { activate<EXACT, decltype(c)::value>(g, a, slope); });
+}
 
 // the three bf16 parts of v by truncation, and hi without infinities and NaN; a NaN keeps a set bit
 __device__ __forceinline__ void split_f32(float v, uint16_t (&p)[kPlanes])
@@ -175,6 +190,86 @@ __device__ __forceinline__ void store_dgu(uint16_t *dgu, int64_t ff_pad, int64_t
                                                        (uint32_t)A::st(v[2]) | (uint32_t)A::st(v[3]) << 16);
         }
     }
+}
+
+// A workgroup's results on their way out: rows of COLS values of type DT in LDS (16 bytes between rows
+// against bank conflicts), then whole 16-byte pieces of rows to memory, consecutive lanes consecutive.
+template <int DT, int COLS> struct Staged {
+    using T = typename Act<DT>::T;
+    static constexpr int kVec = 16 / sizeof(T), kPieces = COLS / kVec;
+    static constexpr uint32_t pitch = COLS * sizeof(T) + 16;
+
+    static __device__ __forceinline__ void put4(unsigned char *lds, int row, int col, const float (&v)[4])
+    {
+        using A = Act<DT>;
+        unsigned char *p = lds + row * pitch + col * sizeof(T);
+        if constexpr (DT == STACR_DTYPE_F32) *reinterpret_cast<float4 *>(p) = make_float4(v[0], v[1], v[2], v[3]);
+        else
+            *reinterpret_cast<uint2 *>(p) = make_uint2((uint32_t)A::st(v[0]) | (uint32_t)A::st(v[1]) << 16,
+                                                       (uint32_t)A::st(v[2]) | (uint32_t)A::st(v[3]) << 16);
+    }
+
+    static __device__ __forceinline__ void get4(const unsigned char *lds, int row, int col, float (&v)[4])
+    {
+        load4<DT>(lds + row * pitch, 0, col, COLS, v, true);
+    }
+
+    // rows m0 .. of `out` (those below M), columns n0 .. (below N)
+    static __device__ __forceinline__ void store(const unsigned char *lds, int rows, int threads, void *out, int64_t ldo,
+                                                 int64_t m0, int64_t M, int64_t n0, int64_t N, bool vec)
+    {
+        const int live = (int)(M - m0 < rows ? M - m0 : rows);
+        T *base = static_cast<T *>(out) + m0 * ldo + n0;
+        const int cols = (int)(N - n0 < COLS ? N - n0 : COLS);
+        for (int i = threadIdx.x; i < live * kPieces; i += threads) {
+            const int r = i / kPieces, c = (i % kPieces) * kVec;
+            const uint4 v = *reinterpret_cast<const uint4 *>(lds + r * pitch + c * sizeof(T));
+            T *p = base + r * ldo + c;
+            if (vec && c + kVec <= cols) {
+                *reinterpret_cast<uint4 *>(p) = v;
+            } else {
+                const T *e = reinterpret_cast<const T *>(lds + r * pitch) + c;
+                for (int k = 0; k < kVec; ++k)
+                    if (c + k < cols) p[k] = e[k];
+            }
+        }
+    }
+
+    // the same rows and columns of `in` into LDS, zeros outside
+    static __device__ __forceinline__ void load(unsigned char *lds, int rows, int threads, const void *in, int64_t ld,
+                                                int64_t m0, int64_t M, int64_t n0, int64_t N, bool vec)
+    {
+        const int live = (int)(M - m0 < rows ? M - m0 : rows);
+        const T *base = static_cast<const T *>(in) + m0 * ld + n0;
+        const int cols = (int)(N - n0 < COLS ? N - n0 : COLS);
+#pragma unroll 4
+        for (int i = threadIdx.x; i < rows * kPieces; i += threads) {
+            const int r = i / kPieces, c = (i % kPieces) * kVec;
+            uint4 v = make_uint4(0, 0, 0, 0);
+            if (r < live) {
+                const T *p = base + r * ld + c;
+                if (vec && c + kVec <= cols) {
+                    v = *reinterpret_cast<const uint4 *>(p);
+                } else {
+                    T e[kVec];
+                    for (int k = 0; k < kVec; ++k) e[k] = c + k < cols ? p[k] : T(0);
+                    __builtin_memcpy(&v, e, 16);
+                }
+            }
+            *reinterpret_cast<uint4 *>(lds + r * pitch + c * sizeof(T)) = v;
+        }
+    }
+};
+
+// LDS of a product's workgroup: two stages, or what its epilogue stages
+template <int DT, int EPI, int BM, int BN> constexpr size_t mm_lds()
+{
+    const size_t stages = 2 * (BM + BN) * 128;
+    size_t out = 0;
+    if (EPI == kFwd) out = BM * Staged<DT, BN / 2>::pitch;
+    if (EPI == kBwd) out = BM * Staged<DT, BN / 2>::pitch * (DT == STACR_DTYPE_F32 ? 1 : 2);
+    if (EPI == kStore) out = BM * Staged<STACR_DTYPE_BF16, BN>::pitch;
+    return out > stages ? out : stages;
 }
 
 // A workgroup's tile: consecutive logical ids share an XCD (ids are dealt to the 8 XCDs round-robin)
@@ -316,67 +411,123 @@ __global__ __launch_bounds__(WM *WN * 64) void k_gated_mm(const MmArgs p)
     }
 
     // a lane holds, of each 16 x 16 block, columns 4 (lane / 16) .. + 3 of row lane % 16
-    const int64_t mfirst = m0 + wm * TM + (lane & 15);
+    constexpr int NT = NW * 64;
+    const int row0 = wm * TM + (lane & 15), quad = (lane >> 4) * 4;
+    __syncthreads();  // the last step has been read
     if constexpr (EPI == kStore) {
+        void *o = half ? p.out2 : p.out;
+        if (p.splits > 1 || p.out_dt == STACR_DTYPE_F32) {
+            float *out = p.splits > 1 ? p.part + ((int64_t)split * p.halves + half) * p.M * p.N : static_cast<float *>(o);
+            const bool vec = p.splits > 1 ? (p.N & 3) == 0 : p.vec;
 #pragma unroll
-        for (int i = 0; i < MI; ++i) {
-            const int64_t m = mfirst + i * 16;
-            if (m >= p.M) continue;
+            for (int i = 0; i < MI; ++i) {
+                const int64_t m = m0 + row0 + i * 16;
+                if (m >= p.M) continue;
 #pragma unroll
-            for (int j = 0; j < NI; ++j) {
-                const int64_t n = n0 + wn * TN + j * 16 + (lane >> 4) * 4;
-                const float v[4] = {acc[i][j][0], acc[i][j][1], acc[i][j][2], acc[i][j][3]};
-                if (p.splits > 1) {
-                    store4<STACR_DTYPE_F32>(p.part, (((int64_t)split * p.halves + half) * p.M + m) * p.N, n, p.N, v,
-                                            (p.N & 3) == 0);
-                } else {
-                    void *o = half ? p.out2 : p.out;
-                    if (p.out_dt == STACR_DTYPE_F32) store4<STACR_DTYPE_F32>(o, m * p.ldo, n, p.N, v, p.vec);
-                    else store4<MT>(o, m * p.ldo, n, p.N, v, p.vec);
+                for (int j = 0; j < NI; ++j) {
+                    const float v[4] = {acc[i][j][0], acc[i][j][1], acc[i][j][2], acc[i][j][3]};
+                    store4<STACR_DTYPE_F32>(out, m * p.N, n0 + wn * TN + j * 16 + quad, p.N, v, vec);
                 }
             }
+        } else {
+            using S = Staged<MT, BN>;
+#pragma unroll
+            for (int i = 0; i < MI; ++i)
+#pragma unroll
+                for (int j = 0; j < NI; ++j) {
+                    const float v[4] = {acc[i][j][0], acc[i][j][1], acc[i][j][2], acc[i][j][3]};
+                    S::put4(lds, row0 + i * 16, wn * TN + j * 16 + quad, v);
+                }
+            __syncthreads();
+            S::store(lds, BM, NT, o, p.ldo, m0, p.M, n0, p.N, p.vec);
         }
     } else {
         constexpr bool EXACT = DT == STACR_DTYPE_F32;
+        constexpr int F = BN / 2;
+        using S = Staged<DT, F>;
+        const int col0 = wn * (TN / 2) + quad;
+        if (p.bias_g || p.bias_u) {
 #pragma unroll
-        for (int j = 0; j < NI; j += 2) {
-            const int64_t f = n0 + (wn * TN + j * 16) / 2 + (lane >> 4) * 4;
-            if (f >= (EPI == kBwd ? p.ff_pad : p.N)) continue;
-            float bg[4] = {}, bu[4] = {};
-            if (p.bias_g) load4<DT>(p.bias_g, 0, f, p.N, bg, false);
-            if (p.bias_u) load4<DT>(p.bias_u, 0, f, p.N, bu, false);
+            for (int j = 0; j < NI; j += 2) {
+                float bg[4] = {}, bu[4] = {};
+                if (p.bias_g) load4<DT>(p.bias_g, 0, n0 + col0 + j * 8, p.N, bg, false);
+                if (p.bias_u) load4<DT>(p.bias_u, 0, n0 + col0 + j * 8, p.N, bu, false);
 #pragma unroll
-            for (int i = 0; i < MI; ++i) {
-                const int64_t m = mfirst + i * 16;
-                if (m >= p.M) continue;
-                float g[4], u[4];
+                for (int i = 0; i < MI; ++i)
 #pragma unroll
-                for (int r = 0; r < 4; ++r) g[r] = acc[i][j][r] + bg[r], u[r] = acc[i][j + 1][r] + bu[r];
-                if constexpr (EPI == kFwd) {
-                    float h[4];
+                    for (int r = 0; r < 4; ++r) acc[i][j][r] += bg[r], acc[i][j + 1][r] += bu[r];
+            }
+        }
+        if constexpr (EPI == kFwd) {
+            with_activation(p.act, [&](auto c) {
 #pragma unroll
-                    for (int r = 0; r < 4; ++r) {
-                        float a, slope;
-                        activate<EXACT>(p.act, g[r], a, slope);
-                        h[r] = a * u[r];
+                for (int i = 0; i < MI; ++i)
+#pragma unroll
+                    for (int j = 0; j < NI; j += 2) {
+                        float h[4];
+#pragma unroll
+                        for (int r = 0; r < 4; ++r) {
+                            float a, slope;
+                            activate<EXACT, decltype(c)::value>(acc[i][j][r], a, slope);
+                            h[r] = a * acc[i][j + 1][r];
+                        }
+                        S::put4(lds, row0 + i * 16, col0 + j * 8, h);
                     }
-                    store4<DT>(p.out, m * p.ldo, f, p.N, h, p.vec);
-                    if (p.gate) {
-                        store4<DT>(p.gate, m * p.ldo, f, p.N, g, p.vec);
-                        store4<DT>(p.up, m * p.ldo, f, p.N, u, p.vec);
-                    }
-                } else {
-                    float d[4], dg[4], du[4];
-                    load4<DT>(p.dh, m * p.ldo, f, p.N, d, p.vec);
+            });
+            __syncthreads();
+            S::store(lds, BM, NT, p.out, p.ldo, m0, p.M, n0, p.N, p.vec);
+            if (p.gate) {  // the kept pre-activations
 #pragma unroll
-                    for (int r = 0; r < 4; ++r) {
-                        float a, slope;
-                        activate<EXACT>(p.act, g[r], a, slope);
-                        dg[r] = d[r] * u[r] * slope;
-                        du[r] = d[r] * a;
-                    }
-                    store_dgu<DT>(p.dgu, p.ff_pad, p.plane, m, f, dg, du);
+                for (int which = 0; which < 2; ++which) {
+                    __syncthreads();
+#pragma unroll
+                    for (int i = 0; i < MI; ++i)
+#pragma unroll
+                        for (int j = 0; j < NI; j += 2) {
+                            const mmf4 &w = acc[i][j + which];
+                            const float v[4] = {w[0], w[1], w[2], w[3]};
+                            S::put4(lds, row0 + i * 16, col0 + j * 8, v);
+                        }
+                    __syncthreads();
+                    S::store(lds, BM, NT, which ? p.up : p.gate, p.ldo, m0, p.M, n0, p.N, p.vec);
                 }
+            }
+        } else {
+            // dh is staged first; a lane's dg takes the place of the dh that it read, du a second stage
+            S::load(lds, BM, NT, p.dh, p.ldo, m0, p.M, n0, p.N, p.vec);
+            __syncthreads();
+            unsigned char *second = lds + BM * S::pitch;
+            with_activation(p.act, [&](auto c) {
+#pragma unroll
+                for (int i = 0; i < MI; ++i) {
+                    __builtin_amdgcn_sched_barrier(0);  // a row of blocks at a time: all at once spill
+                    const int64_t m = m0 + row0 + i * 16;
+#pragma unroll
+                    for (int j = 0; j < NI; j += 2) {
+                        float d[4], dg[4], du[4];
+                        S::get4(lds, row0 + i * 16, col0 + j * 8, d);
+#pragma unroll
+                        for (int r = 0; r < 4; ++r) {
+                            float a, slope;
+                            activate<EXACT, decltype(c)::value>(acc[i][j][r], a, slope);
+                            dg[r] = d[r] * acc[i][j + 1][r] * slope;
+                            du[r] = d[r] * a;
+                        }
+                        if constexpr (EXACT) {
+                            if (m < p.M && n0 + col0 + j * 8 < p.ff_pad)
+                                store_dgu<DT>(p.dgu, p.ff_pad, p.plane, m, n0 + col0 + j * 8, dg, du);
+                        } else {
+                            S::put4(lds, row0 + i * 16, col0 + j * 8, dg);
+                            S::put4(second, row0 + i * 16, col0 + j * 8, du);
+                        }
+                    }
+                }
+            });
+            if constexpr (!EXACT) {
+                __syncthreads();
+#pragma unroll
+                for (int which = 0; which < 2; ++which)
+                    S::store(which ? second : lds, BM, NT, p.dgu + which * p.ff_pad, 2 * p.ff_pad, m0, p.M, n0, p.ff_pad, true);
             }
         }
     }
@@ -618,6 +769,8 @@ inline size_t aligned(size_t n) { return (n + 255) & ~(size_t)255; }
 
 bool aligned_to(const void *p, size_t n) { return (reinterpret_cast<uintptr_t>(p) & (n - 1)) == 0; }
 
+int size_of(int dt) { return dt == STACR_DTYPE_F32 ? 4 : 2; }
+
 struct Problem {
     int dt;
     int64_t rows, d, ff, x_ld;
@@ -647,7 +800,7 @@ template <typename K> void raise_lds(K kernel, size_t bytes)
 template <int DT, bool AK, bool BK, int EPI, int BM, int BN, int WM, int WN>
 void mm_run(MmArgs p, hipStream_t s)
 {
-    constexpr size_t lds = 2 * (BM + BN) * 128;
+    constexpr size_t lds = mm_lds<DT, EPI, BM, BN>();
     static_assert(lds <= 160 * 1024, "LDS budget");
     p.mt = (int)((p.M + BM - 1) / BM);
     const int64_t cols = EPI == kBwd ? p.ff_pad : p.N;
@@ -843,7 +996,7 @@ void product_typed(int dt, MmArgs p, const ProductPlan &plan, float *part, hipSt
     p.splits = plan.splits;
     p.part = part;
     p.out_dt = dt;
-    p.vec = p.N % 4 == 0 && aligned_to(p.out, 16) && aligned_to(p.out2, 16);
+    p.vec = p.N * size_of(dt) % 16 == 0 && aligned_to(p.out, 16) && aligned_to(p.out2, 16);
     p.ldo = p.N;
     if (dt == STACR_DTYPE_F16) product<STACR_DTYPE_F16, AK>(p, s, plan.big);
     else product<STACR_DTYPE_BF16, AK>(p, s, plan.big);
@@ -942,7 +1095,7 @@ int stacr_gated_forward(const void *x, int dtype, int64_t rows, int64_t d, int64
     p.out = h;
     p.gate = gate;
     p.up = up;
-    p.vec = ff % 4 == 0 && aligned_to(h, 16) && aligned_to(gate, 16) && aligned_to(up, 16);
+    p.vec = ff * size_of(dtype) % 16 == 0 && aligned_to(h, 16) && aligned_to(gate, 16) && aligned_to(up, 16);
     dual_typed<kFwd>(dtype, p, s);
     return stacr_hip_check(hipGetLastError(), "gated forward kernels");
 }
@@ -974,7 +1127,7 @@ int stacr_gated_backward(const void *dh, const void *x, int dtype, int64_t rows,
     uint16_t *slopes = dgu ? static_cast<uint16_t *>(dgu) : reinterpret_cast<uint16_t *>(ws + w.dgu);
     float *part = reinterpret_cast<float *>(ws + w.part);
     const Operands o = operands(q, x, w_gate, w_up, ws, w, rows > 0 && (!kept || weights), rows > 0 && (!kept || dx), s);
-    const bool vec = ff % 4 == 0 && aligned_to(dh, 16) && aligned_to(gate, 16) && aligned_to(up, 16);
+    const bool vec = ff * size_of(dtype) % 16 == 0 && aligned_to(dh, 16) && aligned_to(gate, 16) && aligned_to(up, 16);
     if (rows && kept) {
         if (dtype == STACR_DTYPE_F32) slopes_launch<STACR_DTYPE_F32>(dh, gate, up, q, activation, slopes, plane, vec, s);
         else if (dtype == STACR_DTYPE_BF16) slopes_launch<STACR_DTYPE_BF16>(dh, gate, up, q, activation, slopes, plane, vec, s);
