@@ -63,6 +63,14 @@ extern "C" {
 #define STACR_ACT_RELU 3      /* max(g, 0), slope 0 at 0 */
 #define STACR_ACT_SIGMOID 4   /* 1 / (1 + exp(-g)) */
 
+/* rotary positions: which features of a head are a pair, and the scaling of long contexts */
+#define STACR_ROTARY_HALF 0        /* (j, j + rot / 2) */
+#define STACR_ROTARY_INTERLEAVED 1 /* (2 j, 2 j + 1) */
+#define STACR_ROTARY_PLAIN 0
+#define STACR_ROTARY_LINEAR 1
+#define STACR_ROTARY_NTK 2
+#define STACR_ROTARY_BY_PARTS 3
+
 /* status codes */
 #define STACR_OK 0
 #define STACR_ERR_INVALID 1     /* bad argument (shape, dtype, null pointer, size) */
@@ -522,6 +530,46 @@ int stacr_gated_backward(const void *dh, const void *x, int dtype, int64_t rows,
                          int activation, const void *gate, const void *up, void *dx, void *dw_gate, void *dw_up,
                          void *db_gate, void *db_up, void *dgu, void *workspace, size_t workspace_bytes,
                          void *stream);
+
+/*
+ * Tables of rotary positions (no counterpart in the reference): cos and sin, length x rot / 2 fp32, of
+ * p base^(-2 j / rot) for positions p below `length`, computed in 64 bits.  Scaling for contexts longer
+ * than a model was trained on, by `factor` >= 1:
+ *   LINEAR    frequencies divided by the factor
+ *   NTK       base raised to base factor^(rot / (rot - 2))
+ *   BY_PARTS  with n_j the turns of pair j over original_length positions: frequencies as they are where
+ *             n_j > beta_fast, divided by the factor where n_j < beta_slow, a linear blend in j between
+ *             (its ends rounded outwards to whole pairs), and both tables times 0.1 ln(factor) + 1
+ */
+int stacr_rotary_tables(int64_t length, int rot, double base, int scaling, double factor, int64_t original_length,
+                        double beta_fast, double beta_slow, float *cos_t, float *sin_t, void *stream);
+/*
+ * Queries and keys (batch x seq x heads x head, strides of the first three in elements, features
+ * contiguous) turned by their positions' angles: the first `rot` features of each head in pairs
+ * (a, b) -> (a cos - b sin, b cos + a sin), in fp32, rounded once; the others copied.  inverse: by the
+ * negative angle (the gradient).  positions: batch x seq int32 or int64 with two strides (0 repeats),
+ * or NULL for offset + index in the sequence; a position outside the tables' length turns into NaN.
+ * q_out / k_out may be q / k (same strides), and then only the turned features are written; otherwise
+ * they must not overlap.  Either of q, k may have 0 heads.
+ */
+int stacr_rotary(const void *q, const int64_t *q_strides, int q_heads, const void *k, const int64_t *k_strides,
+                 int k_heads, int dtype, int64_t batch, int64_t seq, int head, int rot, int layout,
+                 const float *cos_t, const float *sin_t, int64_t length, const void *positions, int position_bytes,
+                 const int64_t *position_strides, int64_t offset, int inverse, void *q_out,
+                 const int64_t *q_out_strides, void *k_out, const int64_t *k_out_strides, void *stream);
+
+/*
+ * The global norm over `count` gradient tensors and clipping (no counterpart in the reference):
+ *   n = (sum g^2)^(1/2), sum |g| or max |g| over all elements of all tensors (norm_type 2, 1, 0), in 64
+ *   bits; out = g min(1, max_norm / (n + eps)), in fp32, rounded to the tensor's type.
+ * in, out, sizes, dtypes are host arrays (device pointers, elements, type codes; any alignment);
+ * out[i] may be in[i], where nothing is written when the factor is 1, and must not overlap otherwise.
+ * out NULL: the norm alone.  norm: one fp32 on the device.  The same result on every run.
+ */
+int stacr_clip_workspace_bytes(int count, size_t *bytes);
+int stacr_clip_gradients(int count, const void *const *in, void *const *out, const int64_t *sizes, const int *dtypes,
+                         int norm_type, double max_norm, double eps, float *norm, void *workspace,
+                         size_t workspace_bytes, void *stream);
 
 /*
  * Kernel timing (benchmarking aid; no counterpart in the reference).  Between begin and end,

@@ -5,11 +5,13 @@ Drop-in for the reference package's public API (Manar-Hamed/STAC-R, stacr/__init
 include/stacr_amd.h); this package is the host side.
 """
 from .adaptive import AdaptiveSTACRConfig, AdaptiveSTACRLinear, apply_adaptive_stacr, set_stacr_runtime_state
+from .clip import clip_grad_norm, clip_gradients, grad_norm
 from .compressor import STACRCompressor, STACRConfig, stacr_saved_tensors
 from .gated import gated_feed_forward
 from .layers import STACRFunction, STACRLinear
 from .memory import saved_surface_predictor, stacr_stored_bytes
 from .quant import QuantizedValues, quantize_values
+from .rotary_positions import rotary, rotary_tables
 from .surgery import apply_stacr, classify, select_target_names, set_step
 
 __all__ = [
@@ -31,4 +33,9 @@ __all__ = [
     "apply_adaptive_stacr",
     "set_stacr_runtime_state",
     "gated_feed_forward",
+    "rotary",
+    "rotary_tables",
+    "clip_gradients",
+    "clip_grad_norm",
+    "grad_norm",
 ]

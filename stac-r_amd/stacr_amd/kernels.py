@@ -632,3 +632,67 @@ def gated_backward(dh: torch.Tensor, x2d: torch.Tensor | None, w_gate: torch.Ten
                                                 _ptr(dwg), _ptr(dwu), _ptr(dbg), _ptr(dbu), _ptr(dgu), _ptr(ws),
                                                 nbytes, _stream(dev)), "stacr_gated_backward")
     return dx, dwg, dwu, dbg, dbu, dgu
+
+
+# ------------------------------------------------------------------ rotary positions
+def rotary_tables(length: int, rot: int, base: float, scaling: str | None, factor: float, original_length: int,
+                  beta_fast: float, beta_slow: float, device):
+    """(cos, sin), length x rot / 2 fp32 on ``device`` (stacr_rotary_tables)."""
+    cos = torch.empty(length, rot // 2, dtype=torch.float32, device=device)
+    sin = torch.empty_like(cos)
+    _lib.check(_lib.load().stacr_rotary_tables(length, rot, float(base), _lib.ROTARY_SCALINGS[scaling], float(factor),
+                                               int(original_length), float(beta_fast), float(beta_slow), _ptr(cos),
+                                               _ptr(sin), _stream(cos.device)), "stacr_rotary_tables")
+    return cos, sin
+
+
+_Strides = ctypes.c_int64 * 3
+
+
+def rotary(q: torch.Tensor, k: torch.Tensor | None, cos: torch.Tensor, sin: torch.Tensor,
+           positions: torch.Tensor | None, offset: int, layout: str, inverse: bool = False, inplace: bool = False):
+    """Turned q and k (batch x seq x heads x head, any strides; new tensors are contiguous) in one launch
+    (stacr_rotary).  The caller has checked shapes, types and devices (rotary_positions.rotary does)."""
+    batch, seq, heads, head = q.shape
+    if q.stride(3) != 1 and head > 1:
+        q = q.contiguous()
+    if k is not None and k.stride(3) != 1 and head > 1:
+        k = k.contiguous()
+    qo = q if inplace else torch.empty((batch, seq, heads, head), dtype=q.dtype, device=q.device)
+    qs, qos = _Strides(*q.stride()[:3]), _Strides(*qo.stride()[:3])
+    if k is None:
+        ko, ks, kos, kv = None, None, None, 0
+    else:
+        kv = k.shape[2]
+        ko = k if inplace else torch.empty((batch, seq, kv, head), dtype=q.dtype, device=q.device)
+        ks, kos = _Strides(*k.stride()[:3]), _Strides(*ko.stride()[:3])
+    if positions is None:
+        pp, pb, ps = None, 0, None
+    else:
+        pp, pb = _ptr(positions), positions.element_size()
+        ps = _Strides(*((0, positions.stride(0)) if positions.dim() == 1 else positions.stride()))
+    _lib.check(_lib.load().stacr_rotary(_ptr(q), qs, heads, _ptr(k), ks, kv, dtype_code(q.dtype), batch, seq, head,
+                                        2 * cos.shape[1], _lib.ROTARY_LAYOUTS[layout], _ptr(cos), _ptr(sin),
+                                        cos.shape[0], pp, pb, ps, int(offset), int(inverse), _ptr(qo), qos, _ptr(ko),
+                                        kos, _stream(q.device)), "stacr_rotary")
+    return qo, ko
+
+
+# ------------------------------------------------------------------ gradient norm and clipping
+def clip_gradients(grads, outs, norm_type: int, max_norm: float, eps: float, device) -> torch.Tensor:
+    """The global norm (fp32 scalar) of dense tensors, and out = grad * min(1, max_norm / (norm + eps)) into
+    ``outs`` (None: the norm alone), element by element in memory order (stacr_clip_gradients)."""
+    n = len(grads)
+    pointers = ctypes.c_void_p * n
+    L = _lib.load()
+    nbytes = ctypes.c_size_t()
+    _lib.check(L.stacr_clip_workspace_bytes(n, ctypes.byref(nbytes)), "stacr_clip_workspace_bytes")
+    ws = torch.empty(nbytes.value, dtype=torch.uint8, device=device)
+    norm = torch.empty((), dtype=torch.float32, device=device)
+    into = None if outs is None else pointers(*[t.data_ptr() for t in outs])
+    _lib.check(L.stacr_clip_gradients(n, pointers(*[t.data_ptr() for t in grads]), into,
+                                      (ctypes.c_int64 * n)(*[t.numel() for t in grads]),
+                                      (ctypes.c_int * n)(*[DTYPE_CODES[t.dtype] for t in grads]), norm_type,
+                                      float(max_norm), float(eps), _ptr(norm), _ptr(ws), nbytes.value,
+                                      _stream(device)), "stacr_clip_gradients")
+    return norm
