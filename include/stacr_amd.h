@@ -547,7 +547,7 @@ int stacr_rotary_tables(int64_t length, int rot, double base, int scaling, doubl
  * Queries and keys (batch x seq x heads x head, strides of the first three in elements, features
  * contiguous) turned by their positions' angles: the first `rot` features of each head in pairs
  * (a, b) -> (a cos - b sin, b cos + a sin), in fp32, rounded once; the others copied.  inverse: by the
- * negative angle (the gradient).  positions: batch x seq int32 or int64 with two strides (0 repeats),
+ * negative angle (the gradient).  positions: batch x seq int32 or int64 with two strides in elements (0 repeats),
  * or NULL for offset + index in the sequence; a position outside the tables' length turns into NaN.
  * q_out / k_out may be q / k (same strides), and then only the turned features are written; otherwise
  * they must not overlap.  Either of q, k may have 0 heads.
@@ -555,7 +555,7 @@ int stacr_rotary_tables(int64_t length, int rot, double base, int scaling, doubl
 int stacr_rotary(const void *q, const int64_t *q_strides, int q_heads, const void *k, const int64_t *k_strides,
                  int k_heads, int dtype, int64_t batch, int64_t seq, int head, int rot, int layout,
                  const float *cos_t, const float *sin_t, int64_t length, const void *positions, int position_bytes,
-                 const int64_t *position_strides, int64_t offset, int inverse, void *q_out,
+                 int64_t position_stride_batch, int64_t position_stride_seq, int64_t offset, int inverse, void *q_out,
                  const int64_t *q_out_strides, void *k_out, const int64_t *k_out_strides, void *stream);
 
 /*

@@ -220,8 +220,8 @@ int stacr_rotary_tables(int64_t length, int rot, double base, int scaling, doubl
 int stacr_rotary(const void *q, const int64_t *q_strides, int q_heads, const void *k, const int64_t *k_strides, int k_heads,
                  int dtype, int64_t batch, int64_t seq, int head, int rot, int layout, const float *cos_t,
                  const float *sin_t, int64_t length, const void *positions, int position_bytes,
-                 const int64_t *position_strides, int64_t offset, int inverse, void *q_out, const int64_t *q_out_strides,
-                 void *k_out, const int64_t *k_out_strides, void *stream)
+                 int64_t position_stride_batch, int64_t position_stride_seq, int64_t offset, int inverse, void *q_out,
+                 const int64_t *q_out_strides, void *k_out, const int64_t *k_out_strides, void *stream)
 {
     if (dtype != STACR_DTYPE_F32 && dtype != STACR_DTYPE_BF16 && dtype != STACR_DTYPE_F16)
         return stacr_fail(STACR_ERR_INVALID, "stacr_rotary: unsupported dtype code %d", dtype);
@@ -235,7 +235,7 @@ int stacr_rotary(const void *q, const int64_t *q_strides, int q_heads, const voi
         return stacr_fail(STACR_ERR_UNSUPPORTED, "stacr_rotary: more than 2^16 features a head, or 2^20 heads");
     if (batch * seq == 0 || q_heads + k_heads == 0) return STACR_OK;
     if ((q_heads && (!q || !q_out || !q_strides || !q_out_strides)) ||
-        (k_heads && (!k || !k_out || !k_strides || !k_out_strides)) || !cos_t || !sin_t || (positions && !position_strides))
+        (k_heads && (!k || !k_out || !k_strides || !k_out_strides)) || !cos_t || !sin_t)
         return stacr_fail(STACR_ERR_INVALID, "stacr_rotary: NULL pointer argument");
     if (batch * seq > (int64_t)1 << 31)
         return stacr_fail(STACR_ERR_UNSUPPORTED, "stacr_rotary: more than 2^31 tokens");
@@ -269,10 +269,8 @@ int stacr_rotary(const void *q, const int64_t *q_strides, int q_heads, const voi
     a.offset = offset;
     a.pos = positions;
     a.pos_bytes = position_bytes;
-    if (positions) {
-        a.pos_sb = position_strides[0];
-        a.pos_ss = position_strides[1];
-    }
+    a.pos_sb = position_stride_batch;
+    a.pos_ss = position_stride_seq;
     a.head = head;
     a.rot = rot;
     a.sign = inverse ? -1.0f : 1.0f;

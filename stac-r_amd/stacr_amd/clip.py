@@ -35,17 +35,32 @@ def _dense(t) -> bool:
     return True
 
 
-def _check_tensors(grads, name):
-    device = grads[0].device
-    for t in grads:
-        if t.device != device or not t.is_cuda:
-            kernels.require_gpu(t, name)
-            raise RuntimeError(f"{name} are on {device} and {t.device}: one GPU is needed")
-        if t.dtype not in kernels.DTYPE_CODES:
-            kernels.dtype_code(t.dtype)
+def _refuse(tensors, name):
+    """Says what is wrong with the first tensor that is."""
+    device = tensors[0].device
+    for t in tensors:
         if t.layout != torch.strided:
             raise ValueError(f"{name} must be dense tensors, got {t.layout}")
-    return device
+        kernels.require_gpu(t, name)
+        kernels.dtype_code(t.dtype)
+        if t.device != device:
+            raise RuntimeError(f"{name} are on {device} and {t.device}: one GPU is needed")
+
+
+def _facts(tensors, name):
+    """(addresses, element counts, type codes) of tensors on one GPU; None for the tensors' own order if every
+    one is contiguous, else the list of those that are."""
+    codes = kernels.DTYPE_CODES
+    try:
+        index = tensors[0].get_device()
+        if index < 0 or any([t.get_device() != index for t in tensors]):
+            _refuse(tensors, name)
+        types = [codes[t.dtype] for t in tensors]
+        plain = [t.is_contiguous() for t in tensors]
+        return [t.data_ptr() for t in tensors], [t.numel() for t in tensors], types, None if all(plain) else plain
+    except (KeyError, RuntimeError):
+        _refuse(tensors, name)
+        raise
 
 
 def clip_gradients(grads: Iterable[torch.Tensor], max_norm: float, *, norm_type: float = 2.0, eps: float = 1e-6,
@@ -68,36 +83,36 @@ def clip_gradients(grads: Iterable[torch.Tensor], max_norm: float, *, norm_type:
             raise ValueError(f"{len(grads)} gradients and {len(out)} outputs")
     if not grads:
         return torch.zeros(())
-    device = _check_tensors(grads, "gradients")
+    at, sizes, codes, plain = _facts(grads, "gradients")
+    device = grads[0].device
+    into, copies = at, []
     if out is not None:
-        if _check_tensors(out, "outputs") != device:
+        into, _, out_codes, out_plain = _facts(out, "outputs")
+        if out[0].device != device:
             raise RuntimeError(f"gradients are on {device}, outputs on {out[0].device}")
-        for g, o in zip(grads, out):
-            if g.shape != o.shape or g.dtype != o.dtype:
-                raise ValueError(f"an output of {tuple(o.shape)} {o.dtype} for a gradient of {tuple(g.shape)} {g.dtype}")
+        if codes != out_codes or [g.shape for g in grads] != [o.shape for o in out]:
+            for g, o in zip(grads, out):
+                if g.shape != o.shape or g.dtype != o.dtype:
+                    raise ValueError(f"an output of {tuple(o.shape)} {o.dtype} for a gradient of {tuple(g.shape)} {g.dtype}")
+        plain = plain or out_plain
     if error_if_nonfinite:
         total = grad_norm(grads, norm_type=norm_type)
         if not math.isfinite(float(total)):
             raise RuntimeError(f"The total norm of the gradients is {float(total)}: it cannot be clipped")
-    # elements are taken in memory order: a tensor with gaps goes through a packed copy
-    with torch.no_grad():
-        into = grads if out is None else out
-        src, dst, copies = [], [], []
-        for g, o in zip(grads, into):
-            if _dense(g) and (o is g or o.stride() == g.stride()):
-                src.append(g)
-                dst.append(o)
-                continue
-            if o is g and any(s == 0 and n > 1 for s, n in zip(g.stride(), g.shape)):
-                raise ValueError("a gradient whose elements share memory cannot be scaled in place")
-            packed = g.contiguous() if _dense(o) and o.is_contiguous() else g.clone(memory_format=torch.contiguous_format)
-            src.append(packed)
-            if o.is_contiguous():
-                dst.append(o)
-            else:
-                dst.append(packed)
+    if plain is not None:
+        # elements are taken in memory order: a tensor with gaps goes through a packed copy
+        at, into = list(at), list(into)
+        with torch.no_grad():
+            for i, (g, o) in enumerate(zip(grads, grads if out is None else out)):
+                if _dense(g) and o.stride() == g.stride():
+                    continue
+                if o is g and any(s == 0 and n > 1 for s, n in zip(g.stride(), g.shape)):
+                    raise ValueError("a gradient whose elements share memory cannot be scaled in place")
+                packed = g.clone(memory_format=torch.contiguous_format)
+                at[i] = into[i] = packed.data_ptr()
                 copies.append((o, packed))
-        norm = kernels.clip_gradients(src, dst, code, max_norm, eps, device)
+    norm = kernels.clip_gradients(at, into, sizes, codes, code, max_norm, eps, device)
+    with torch.no_grad():
         for o, packed in copies:
             o.copy_(packed)
     return norm
@@ -109,9 +124,12 @@ def grad_norm(grads: Iterable[torch.Tensor], *, norm_type: float = 2.0) -> torch
     code = _norm_code(norm_type)
     if not grads:
         return torch.zeros(())
-    device = _check_tensors(grads, "gradients")
-    with torch.no_grad():
-        return kernels.clip_gradients([g if _dense(g) else g.contiguous() for g in grads], None, code, 0.0, 0.0, device)
+    at, sizes, codes, plain = _facts(grads, "gradients")
+    if plain is not None:
+        with torch.no_grad():
+            grads = [g if _dense(g) else g.contiguous() for g in grads]
+        at = [g.data_ptr() for g in grads]
+    return kernels.clip_gradients(at, None, sizes, codes, code, 0.0, 0.0, grads[0].device)
 
 
 def clip_grad_norm(parameters: torch.Tensor | Iterable[torch.Tensor], max_norm: float, *, norm_type: float = 2.0,

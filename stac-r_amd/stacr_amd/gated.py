@@ -18,21 +18,22 @@ def _check_gated(x, w_gate, w_up, b_gate, b_up, activation) -> None:
     if activation not in _lib.ACTIVATION_CODES:
         raise ValueError(f"activation must be one of {list(ACTIVATIONS)}, got {activation!r}")
     kernels.require_gpu(x, "input")
-    if w_gate.dim() != 2 or w_gate.shape != w_up.shape or 0 in w_gate.shape:
-        raise ValueError(f"w_gate and w_up must be two (ff, d) matrices of one shape, got {tuple(w_gate.shape)} and "
+    shape = w_gate.shape
+    if len(shape) != 2 or shape != w_up.shape or 0 in shape:
+        raise ValueError(f"w_gate and w_up must be two (ff, d) matrices of one shape, got {tuple(shape)} and "
                          f"{tuple(w_up.shape)}")
-    ff, d = w_gate.shape
-    if x.dim() < 1 or x.shape[-1] != d:
-        raise ValueError(f"Expected last input dimension {d}, got {tuple(x.shape)}")
+    if x.dim() < 1 or x.shape[-1] != shape[1]:
+        raise ValueError(f"Expected last input dimension {shape[1]}, got {tuple(x.shape)}")
+    dtype, index = x.dtype, x.get_device()
     for name, t in (("w_gate", w_gate), ("w_up", w_up), ("b_gate", b_gate), ("b_up", b_up)):
         if t is None:
             continue
-        if t.device != x.device:
+        if t.get_device() != index:
             raise RuntimeError(f"{name} is on {t.device}, the input on {x.device}")
-        if t.dtype != x.dtype:
-            raise TypeError(f"{name} is {t.dtype}, the input {x.dtype}: one type throughout")
-        if name[0] == "b" and t.shape != (ff,):
-            raise ValueError(f"{name} must have {ff} values, got shape {tuple(t.shape)}")
+        if t.dtype != dtype:
+            raise TypeError(f"{name} is {t.dtype}, the input {dtype}: one type throughout")
+        if name[0] == "b" and t.shape != shape[:1]:
+            raise ValueError(f"{name} must have {shape[0]} values, got shape {tuple(t.shape)}")
 
 
 def _contiguous(t):
@@ -79,9 +80,11 @@ def gated_feed_forward(x: torch.Tensor, w_gate: torch.Tensor, w_up: torch.Tensor
                                     (b_gate is not None and b_gate.requires_grad) or
                                     (b_up is not None and b_up.requires_grad)):
         return GatedFeedForwardFunction.apply(x, w_gate, w_up, b_gate, b_up, activation)
+    if x.dim() == 2:
+        return kernels.gated_forward(x, w_gate, w_up, _contiguous(b_gate), _contiguous(b_up), activation)
     h = kernels.gated_forward(x.reshape(-1, x.shape[-1]), w_gate, w_up, _contiguous(b_gate), _contiguous(b_up),
                               activation)
-    return h if x.dim() == 2 else h.view(*x.shape[:-1], h.shape[1])
+    return h.view(*x.shape[:-1], h.shape[1])
 
 
 __all__ = ["ACTIVATIONS", "GatedFeedForwardFunction", "gated_feed_forward"]

@@ -6,6 +6,7 @@ arithmetic has no CPU implementation in this package.
 from __future__ import annotations
 
 import ctypes
+from array import array
 
 import torch
 
@@ -566,26 +567,41 @@ def c1_restore(coeff: torch.Tensor, scales: torch.Tensor | None, basis: torch.Te
 
 
 # ------------------------------------------------------------------ gated feed-forward block
-def _gated_workspace(x2d, dtype, rows, d, x_ld, w_gate, w_up, backward):
+# The calls from here on serve single tokens too, where the host's time is the call's: addresses go as
+# plain integers (ctypes converts them faster than c_void_p objects), the stream by its raw handle.
+def _at(t: torch.Tensor | None) -> int | None:
+    return None if t is None else t.data_ptr()
+
+
+def _raw_stream(t: torch.Tensor) -> int:
+    return torch._C._cuda_getCurrentRawStream(t.get_device())
+
+
+# Rows up to which the forward runs without a workspace (the library's few-row form).
+GATED_FEW_ROWS = 64
+
+
+def _gated_workspace(x2d, code, rows, d, x_ld, w_gate, w_up, backward):
     nbytes = ctypes.c_size_t()
-    _lib.check(_lib.load().stacr_gated_workspace_bytes(_ptr(x2d), dtype_code(dtype), rows, d, x_ld, _ptr(w_gate),
-                                                       _ptr(w_up), w_gate.shape[0], int(backward),
-                                                       ctypes.byref(nbytes)), "stacr_gated_workspace_bytes")
+    rc = _lib.load().stacr_gated_workspace_bytes(_at(x2d), code, rows, d, x_ld, w_gate.data_ptr(), w_up.data_ptr(),
+                                                 w_gate.shape[0], backward, ctypes.byref(nbytes))
+    if rc:
+        _lib.check(rc, "stacr_gated_workspace_bytes")
     if not nbytes.value:
         return None, 0
     return torch.empty(nbytes.value, dtype=torch.uint8, device=w_gate.device), nbytes.value
 
 
 def _rows_of(x2d):
-    """A matrix whose rows are contiguous (any row stride of at least the row's length, up to the library's limit); a single row's
-    stride, which means nothing, is its length."""
+    """A matrix whose rows are contiguous, and their stride: any of at least the row's length, up to the
+    library's limit (a single row's stride means nothing)."""
     rows, d = x2d.shape
-    if x2d.stride(1) == 1 or d == 1:
-        if d <= x2d.stride(0) <= 1 << 20 and rows > 1:
-            return x2d
-        if rows <= 1:
-            return x2d.as_strided((rows, d), (d, 1))
-    return x2d.contiguous()
+    ld, one = x2d.stride()
+    if rows <= 1:
+        ld = d
+    if (one != 1 and d > 1) or not d <= ld <= 1 << 20:
+        return x2d.contiguous(), d
+    return x2d, ld
 
 
 def gated_forward(x2d: torch.Tensor, w_gate: torch.Tensor, w_up: torch.Tensor, b_gate: torch.Tensor | None = None,
@@ -593,16 +609,19 @@ def gated_forward(x2d: torch.Tensor, w_gate: torch.Tensor, w_up: torch.Tensor, b
     """h = act(x Wg^T + bg) * (x Wu^T + bu) of rows x d (stacr_gated_forward); with ``keep`` (h, g, u), the
     pre-activations rounded to the type.  The caller has checked shapes, types and devices
     (gated.gated_feed_forward does)."""
-    x2d, w_gate, w_up = _rows_of(x2d), w_gate.contiguous(), w_up.contiguous()
+    x2d, x_ld = _rows_of(x2d)
+    w_gate, w_up = w_gate.contiguous(), w_up.contiguous()
     rows, d = x2d.shape
     ff = w_gate.shape[0]
-    h = torch.empty(rows, ff, dtype=x2d.dtype, device=x2d.device)
+    code = dtype_code(x2d.dtype)
+    h = x2d.new_empty((rows, ff))
     gate, up = (torch.empty_like(h), torch.empty_like(h)) if keep else (None, None)
-    ws, nbytes = _gated_workspace(x2d, x2d.dtype, rows, d, x2d.stride(0), w_gate, w_up, False)
-    _lib.check(_lib.load().stacr_gated_forward(_ptr(x2d), dtype_code(x2d.dtype), rows, d, x2d.stride(0), _ptr(w_gate),
-                                               _ptr(w_up), ff, _ptr(b_gate), _ptr(b_up),
-                                               _lib.ACTIVATION_CODES[activation], _ptr(h), _ptr(gate), _ptr(up),
-                                               _ptr(ws), nbytes, _stream(x2d.device)), "stacr_gated_forward")
+    ws, nbytes = (None, 0) if rows <= GATED_FEW_ROWS else _gated_workspace(x2d, code, rows, d, x_ld, w_gate, w_up, 0)
+    rc = _lib.load().stacr_gated_forward(x2d.data_ptr(), code, rows, d, x_ld, w_gate.data_ptr(), w_up.data_ptr(), ff,
+                                         _at(b_gate), _at(b_up), _lib.ACTIVATION_CODES[activation], h.data_ptr(),
+                                         _at(gate), _at(up), _at(ws), nbytes, _raw_stream(x2d))
+    if rc:
+        _lib.check(rc, "stacr_gated_forward")
     return (h, gate, up) if keep else h
 
 
@@ -615,22 +634,22 @@ def gated_backward(dh: torch.Tensor, x2d: torch.Tensor | None, w_gate: torch.Ten
     out dgu = [dg | du], rows x 2 p with p = ff rounded up to 8 (16-bit types)."""
     dh, w_gate, w_up = dh.contiguous(), w_gate.contiguous(), w_up.contiguous()
     rows, ff = dh.shape
-    d, dtype, dev = w_gate.shape[1], dh.dtype, dh.device
-    if x2d is not None:
-        x2d = _rows_of(x2d)
-    dx = torch.empty(rows, d, dtype=dtype, device=dev) if needs[0] else None
+    d = w_gate.shape[1]
+    code = dtype_code(dh.dtype)
+    x2d, x_ld = _rows_of(x2d) if x2d is not None else (None, d)
+    dx = dh.new_empty((rows, d)) if needs[0] else None
     dwg, dwu = (torch.empty_like(w_gate), torch.empty_like(w_up)) if needs[1] else (None, None)
-    dbg = torch.empty(ff, dtype=dtype, device=dev) if needs[2] else None
-    dbu = torch.empty(ff, dtype=dtype, device=dev) if needs[3] else None
-    dgu = torch.empty(rows, 2 * ((ff + 7) // 8 * 8), dtype=dtype, device=dev) if slopes else None
+    dbg = dh.new_empty(ff) if needs[2] else None
+    dbu = dh.new_empty(ff) if needs[3] else None
+    dgu = dh.new_empty((rows, 2 * ((ff + 7) // 8 * 8))) if slopes else None
     gate, up = kept if kept is not None else (None, None)
-    x_ld = x2d.stride(0) if x2d is not None else d
-    ws, nbytes = _gated_workspace(x2d, dtype, rows, d, x_ld, w_gate, w_up, True)
-    _lib.check(_lib.load().stacr_gated_backward(_ptr(dh), _ptr(x2d), dtype_code(dtype), rows, d, x_ld, _ptr(w_gate),
-                                                _ptr(w_up), ff, _ptr(b_gate), _ptr(b_up),
-                                                _lib.ACTIVATION_CODES[activation], _ptr(gate), _ptr(up), _ptr(dx),
-                                                _ptr(dwg), _ptr(dwu), _ptr(dbg), _ptr(dbu), _ptr(dgu), _ptr(ws),
-                                                nbytes, _stream(dev)), "stacr_gated_backward")
+    ws, nbytes = _gated_workspace(x2d, code, rows, d, x_ld, w_gate, w_up, 1)
+    rc = _lib.load().stacr_gated_backward(dh.data_ptr(), _at(x2d), code, rows, d, x_ld, w_gate.data_ptr(),
+                                          w_up.data_ptr(), ff, _at(b_gate), _at(b_up),
+                                          _lib.ACTIVATION_CODES[activation], _at(gate), _at(up), _at(dx), _at(dwg),
+                                          _at(dwu), _at(dbg), _at(dbu), _at(dgu), _at(ws), nbytes, _raw_stream(dh))
+    if rc:
+        _lib.check(rc, "stacr_gated_backward")
     return dx, dwg, dwu, dbg, dbu, dgu
 
 
@@ -646,7 +665,7 @@ def rotary_tables(length: int, rot: int, base: float, scaling: str | None, facto
     return cos, sin
 
 
-_Strides = ctypes.c_int64 * 3
+_Strides = ctypes.c_int64 * 12
 
 
 def rotary(q: torch.Tensor, k: torch.Tensor | None, cos: torch.Tensor, sin: torch.Tensor,
@@ -654,45 +673,54 @@ def rotary(q: torch.Tensor, k: torch.Tensor | None, cos: torch.Tensor, sin: torc
     """Turned q and k (batch x seq x heads x head, any strides; new tensors are contiguous) in one launch
     (stacr_rotary).  The caller has checked shapes, types and devices (rotary_positions.rotary does)."""
     batch, seq, heads, head = q.shape
-    if q.stride(3) != 1 and head > 1:
+    qs = q.stride()
+    if qs[3] != 1 and head > 1:
         q = q.contiguous()
-    if k is not None and k.stride(3) != 1 and head > 1:
-        k = k.contiguous()
-    qo = q if inplace else torch.empty((batch, seq, heads, head), dtype=q.dtype, device=q.device)
-    qs, qos = _Strides(*q.stride()[:3]), _Strides(*qo.stride()[:3])
+        qs = q.stride()
+    qo, qos = (q, qs) if inplace else (q.new_empty((batch, seq, heads, head)), (seq * heads * head, heads * head, head))
     if k is None:
-        ko, ks, kos, kv = None, None, None, 0
+        ko, kp, kop, kv, ks, kos = None, None, None, 0, qs, qos
     else:
-        kv = k.shape[2]
-        ko = k if inplace else torch.empty((batch, seq, kv, head), dtype=q.dtype, device=q.device)
-        ks, kos = _Strides(*k.stride()[:3]), _Strides(*ko.stride()[:3])
+        kv, ks = k.shape[2], k.stride()
+        if ks[3] != 1 and head > 1:
+            k = k.contiguous()
+            ks = k.stride()
+        ko, kos = (k, ks) if inplace else (k.new_empty((batch, seq, kv, head)), (seq * kv * head, kv * head, head))
+        kp, kop = k.data_ptr(), ko.data_ptr()
+    # one array: the strides of q, k and their results, three each
+    strides = _Strides(qs[0], qs[1], qs[2], ks[0], ks[1], ks[2], qos[0], qos[1], qos[2], kos[0], kos[1], kos[2])
+    at = ctypes.addressof(strides)
     if positions is None:
-        pp, pb, ps = None, 0, None
+        pp, pb, sb, ss = None, 0, 0, 0
     else:
-        pp, pb = _ptr(positions), positions.element_size()
-        ps = _Strides(*((0, positions.stride(0)) if positions.dim() == 1 else positions.stride()))
-    _lib.check(_lib.load().stacr_rotary(_ptr(q), qs, heads, _ptr(k), ks, kv, dtype_code(q.dtype), batch, seq, head,
-                                        2 * cos.shape[1], _lib.ROTARY_LAYOUTS[layout], _ptr(cos), _ptr(sin),
-                                        cos.shape[0], pp, pb, ps, int(offset), int(inverse), _ptr(qo), qos, _ptr(ko),
-                                        kos, _stream(q.device)), "stacr_rotary")
+        pp, pb = positions.data_ptr(), positions.element_size()
+        sb, ss = (0, positions.stride(0)) if positions.dim() == 1 else positions.stride()
+    rc = _lib.load().stacr_rotary(q.data_ptr(), at, heads, kp, at + 24, kv, dtype_code(q.dtype), batch, seq, head,
+                                  2 * cos.shape[1], _lib.ROTARY_LAYOUTS[layout], cos.data_ptr(), sin.data_ptr(),
+                                  cos.shape[0], pp, pb, sb, ss, offset, inverse, qo.data_ptr(), at + 48, kop, at + 72,
+                                  _raw_stream(q))
+    if rc:
+        _lib.check(rc, "stacr_rotary")
     return qo, ko
 
 
 # ------------------------------------------------------------------ gradient norm and clipping
-def clip_gradients(grads, outs, norm_type: int, max_norm: float, eps: float, device) -> torch.Tensor:
-    """The global norm (fp32 scalar) of dense tensors, and out = grad * min(1, max_norm / (norm + eps)) into
-    ``outs`` (None: the norm alone), element by element in memory order (stacr_clip_gradients)."""
-    n = len(grads)
-    pointers = ctypes.c_void_p * n
+def clip_gradients(pointers, out_pointers, sizes, codes, norm_type: int, max_norm: float, eps: float,
+                   device) -> torch.Tensor:
+    """The global norm (fp32 scalar) of dense tensors, and out = grad * min(1, max_norm / (norm + eps)), element
+    by element in memory order (stacr_clip_gradients).  The tensors come as lists of addresses, element counts
+    and type codes; ``out_pointers`` None: the norm alone."""
+    n = len(pointers)
     L = _lib.load()
     nbytes = ctypes.c_size_t()
     _lib.check(L.stacr_clip_workspace_bytes(n, ctypes.byref(nbytes)), "stacr_clip_workspace_bytes")
     ws = torch.empty(nbytes.value, dtype=torch.uint8, device=device)
     norm = torch.empty((), dtype=torch.float32, device=device)
-    into = None if outs is None else pointers(*[t.data_ptr() for t in outs])
-    _lib.check(L.stacr_clip_gradients(n, pointers(*[t.data_ptr() for t in grads]), into,
-                                      (ctypes.c_int64 * n)(*[t.numel() for t in grads]),
-                                      (ctypes.c_int * n)(*[DTYPE_CODES[t.dtype] for t in grads]), norm_type,
-                                      float(max_norm), float(eps), _ptr(norm), _ptr(ws), nbytes.value,
-                                      _stream(device)), "stacr_clip_gradients")
+    src, counts, types = array("Q", pointers), array("q", sizes), array("i", codes)
+    dst = None if out_pointers is None else (src if out_pointers is pointers else array("Q", out_pointers))
+    rc = L.stacr_clip_gradients(n, src.buffer_info()[0], None if dst is None else dst.buffer_info()[0],
+                                counts.buffer_info()[0], types.buffer_info()[0], norm_type, max_norm, eps,
+                                norm.data_ptr(), ws.data_ptr(), nbytes.value, _raw_stream(norm))
+    if rc:
+        _lib.check(rc, "stacr_clip_gradients")
     return norm

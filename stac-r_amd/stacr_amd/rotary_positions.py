@@ -64,8 +64,9 @@ def _check_rotary(q, k, cos, sin, positions, layout) -> None:
             raise TypeError(f"positions must be int32 or int64, got {positions.dtype}")
         if positions.shape not in ((q.shape[1],), (q.shape[0], q.shape[1])):
             raise ValueError(f"positions must be (seq,) or (batch, seq), got {tuple(positions.shape)}")
+    index = q.get_device()
     for t in (k, cos, sin, positions):
-        if t is not None and t.device != q.device:
+        if t is not None and t.get_device() != index:
             raise RuntimeError(f"rotary: tensors on {t.device} and {q.device}")
 
 

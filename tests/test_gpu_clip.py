@@ -218,3 +218,6 @@ class _Elsewhere:
 
     def __init__(self, like):
         self.device, self.is_cuda, self.dtype, self.layout = torch.device("cuda:1"), True, like.dtype, like.layout
+
+    def get_device(self):
+        return 1
