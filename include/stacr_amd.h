@@ -504,7 +504,9 @@ int stacr_qr_tall(const float *a, int64_t rows, int cols, float *q, float *r, vo
  * Gated feed-forward block (no counterpart in the reference, whose layers wrap its projections):
  *   g = x Wg^T + bg, u = x Wu^T + bu, h = act(g) * u
  * x: rows x d with rows x_ld >= d values apart; w_gate, w_up: ff x d (row-major, as nn.Linear keeps
- * them); biases ff values or NULL; h (and gate, up: g and u rounded, both or neither): rows x ff.  One
+ * them); biases ff values or NULL; h: rows x ff.  gate and up (both or NULL; rows x ff) keep g and u for
+ * the backward: rounded to the type, or with gate_low and up_low (bytes, rows x ff; 16-bit types) in 24
+ * bits, the upper 16 bits of the fp32 value in gate / up and the next 8 in the low bytes.  One
  * type throughout; sums in fp32 (fp32 inputs: to fp32 accuracy).  The workspace holds operands whose
  * rows are not whole, aligned groups of 8 values in another form (fp32: always), so its size depends on
  * the pointers' alignment, which is all that the query looks at.  rows 0 is a no-op.  d, ff and x_ld at
@@ -514,7 +516,8 @@ int stacr_gated_workspace_bytes(const void *x, int dtype, int64_t rows, int64_t 
                                 const void *w_up, int64_t ff, int backward, size_t *bytes);
 int stacr_gated_forward(const void *x, int dtype, int64_t rows, int64_t d, int64_t x_ld, const void *w_gate,
                         const void *w_up, int64_t ff, const void *b_gate, const void *b_up, int activation, void *h,
-                        void *gate, void *up, void *workspace, size_t workspace_bytes, void *stream);
+                        void *gate, void *up, void *gate_low, void *up_low, void *workspace, size_t workspace_bytes,
+                        void *stream);
 /*
  * Its gradients for dh (rows x ff): dg = dh u act'(g), du = dh act(g), dx = dg Wg + du Wu (rows x d),
  * dW_gate = dg^T x, dW_up = du^T x (ff x d), db = column sums.  gate and up as the forward kept them, or
@@ -527,8 +530,8 @@ int stacr_gated_forward(const void *x, int dtype, int64_t rows, int64_t d, int64
  */
 int stacr_gated_backward(const void *dh, const void *x, int dtype, int64_t rows, int64_t d, int64_t x_ld,
                          const void *w_gate, const void *w_up, int64_t ff, const void *b_gate, const void *b_up,
-                         int activation, const void *gate, const void *up, void *dx, void *dw_gate, void *dw_up,
-                         void *db_gate, void *db_up, void *dgu, void *workspace, size_t workspace_bytes,
+                         int activation, const void *gate, const void *up, const void *gate_low, const void *up_low,
+                         void *dx, void *dw_gate, void *dw_up, void *db_gate, void *db_up, void *dgu, void *workspace, size_t workspace_bytes,
                          void *stream);
 
 /*

@@ -8,7 +8,8 @@
 //
 // Tensors come as pointers and lengths in the kernel's own arguments (4 KiB: about 120 tensors a
 // launch), so nothing is copied to the device and a call can be captured into a graph.  The tensors
-// are cut into chunks of 8192 elements and a workgroup takes a range of chunks.
+// are cut into chunks of 8192 elements and a workgroup takes a range of chunks, so of each tensor one
+// run of elements; a chunk's loads are under way while the one before it is worked on.
 #include "internal.h"
 
 using namespace stacr;
@@ -25,10 +26,9 @@ struct ClipArgs {
     void *out[kTensors];
     int64_t n[kTensors];
     uint32_t first[kTensors];           // first chunk of the tensor in this launch
-    uint8_t dtype[kTensors];
+    uint32_t dtype[kTensors];
     int count;
     uint32_t chunks;
-    int norm;                           // 0: max, 1, 2
     int parts;                          // partial norms over all launches
     double *part;                       // the norm pass: this launch's
     double max_norm, eps;
@@ -36,13 +36,51 @@ struct ClipArgs {
 };
 static_assert(sizeof(ClipArgs) <= 4096, "kernel arguments");
 
+struct Raw8 {  // eight elements as they lie in memory
+    uint4 w[2];
+};
+
 // eight elements from p on, at any alignment
-template <int DT> __device__ __forceinline__ void load8(const typename Act<DT>::T *p, float (&v)[8])
+template <int DT> __device__ __forceinline__ Raw8 load8(const typename Act<DT>::T *p)
+{
+    Raw8 r;
+    __builtin_memcpy(&r.w, p, 8 * sizeof(*p));
+    return r;
+}
+
+template <int DT> __device__ __forceinline__ void widen(const Raw8 &r, float (&v)[8])
 {
     typename Act<DT>::T e[8];
-    __builtin_memcpy(e, p, sizeof(e));
+    __builtin_memcpy(e, &r.w, sizeof(e));
 #pragma unroll
     for (int k = 0; k < 8; ++k) v[k] = Act<DT>::ld(e[k]);
+}
+
+// body(values, first element's offset) over the whole chunks of elements [from, to), two chunks under way;
+// returns where the rest begins
+template <int DT, typename F>
+__device__ __forceinline__ int64_t whole_chunks(const typename Act<DT>::T *p, int64_t from, int64_t to, F &&body)
+{
+    const int mine = threadIdx.x * 8;
+    if (to - from < kChunk) return from;
+    Raw8 r[kPieces], next[kPieces];
+#pragma unroll
+    for (int i = 0; i < kPieces; ++i) r[i] = load8<DT>(p + from + i * kBlock * 8 + mine);
+    for (; to - from >= kChunk; from += kChunk) {
+        const bool more = to - from >= 2 * kChunk;
+        if (more) {
+#pragma unroll
+            for (int i = 0; i < kPieces; ++i) next[i] = load8<DT>(p + from + kChunk + i * kBlock * 8 + mine);
+        }
+#pragma unroll
+        for (int i = 0; i < kPieces; ++i) {
+            float v[8];
+            widen<DT>(r[i], v);
+            body(v, from + i * kBlock * 8 + mine);
+            if (more) r[i] = next[i];
+        }
+    }
+    return from;
 }
 
 template <int NORM> __device__ __forceinline__ void take(double &sum, uint32_t &top, float v)
@@ -56,70 +94,66 @@ template <int NORM> __device__ __forceinline__ void take(double &sum, uint32_t &
 }
 
 template <int DT, int NORM>
-__device__ __forceinline__ void chunk_norm(const void *in, int64_t n, int64_t start, double &sum, uint32_t &top)
+__device__ __forceinline__ void run_norm(const void *in, int64_t from, int64_t to, double &sum, uint32_t &top)
 {
-    const typename Act<DT>::T *p = static_cast<const typename Act<DT>::T *>(in) + start;
-    const int64_t left = n - start;
-    if (left >= kChunk) {
-        float v[kPieces][8];
+    const typename Act<DT>::T *p = static_cast<const typename Act<DT>::T *>(in);
+    from = whole_chunks<DT>(p, from, to, [&](const float(&v)[8], int64_t) {
 #pragma unroll
-        for (int i = 0; i < kPieces; ++i) load8<DT>(p + (i * kBlock + threadIdx.x) * 8, v[i]);
+        for (int k = 0; k < 8; ++k) take<NORM>(sum, top, v[k]);
+    });
+    for (int64_t i = from + threadIdx.x * 8; i < to; i += kBlock * 8) {
+        if (i + 8 <= to) {
+            float v[8];
+            widen<DT>(load8<DT>(p + i), v);
 #pragma unroll
-        for (int i = 0; i < kPieces; ++i)
-#pragma unroll
-            for (int k = 0; k < 8; ++k) take<NORM>(sum, top, v[i][k]);
-    } else {
-        for (int i = threadIdx.x * 8; i < left; i += kBlock * 8) {
-            if (i + 8 <= left) {
-                float v[8];
-                load8<DT>(p + i, v);
-#pragma unroll
-                for (int k = 0; k < 8; ++k) take<NORM>(sum, top, v[k]);
-            } else {
-                for (int k = i; k < left; ++k) take<NORM>(sum, top, Act<DT>::ld(p[k]));
-            }
+            for (int k = 0; k < 8; ++k) take<NORM>(sum, top, v[k]);
+        } else {
+            for (int64_t k = i; k < to; ++k) take<NORM>(sum, top, Act<DT>::ld(p[k]));
         }
     }
 }
 
 template <int DT>
-__device__ __forceinline__ void chunk_scale(const void *in, void *out, int64_t n, int64_t start, float f)
+__device__ __forceinline__ void run_scale(const void *in, void *out, int64_t from, int64_t to, float f)
 {
     using T = typename Act<DT>::T;
-    const T *p = static_cast<const T *>(in) + start;
-    T *q = static_cast<T *>(out) + start;
-    const int64_t left = n - start;
-    if (left >= kChunk) {
-        float v[kPieces][8];
+    const T *p = static_cast<const T *>(in);
+    T *q = static_cast<T *>(out);
+    const auto put = [&](const float(&v)[8], int64_t at) {
+        T e[8];
 #pragma unroll
-        for (int i = 0; i < kPieces; ++i) load8<DT>(p + (i * kBlock + threadIdx.x) * 8, v[i]);
-#pragma unroll
-        for (int i = 0; i < kPieces; ++i) {
-            T e[8];
-#pragma unroll
-            for (int k = 0; k < 8; ++k) e[k] = Act<DT>::st(v[i][k] * f);
-            __builtin_memcpy(q + (i * kBlock + threadIdx.x) * 8, e, sizeof(e));
+        for (int k = 0; k < 8; ++k) e[k] = Act<DT>::st(v[k] * f);
+        __builtin_memcpy(q + at, e, sizeof(e));
+    };
+    from = whole_chunks<DT>(p, from, to, put);
+    for (int64_t i = from + threadIdx.x * 8; i < to; i += kBlock * 8) {
+        if (i + 8 <= to) {
+            float v[8];
+            widen<DT>(load8<DT>(p + i), v);
+            put(v, i);
+        } else {
+            for (int64_t k = i; k < to; ++k) q[k] = Act<DT>::st(Act<DT>::ld(p[k]) * f);
         }
-    } else {
-        for (int64_t i = threadIdx.x; i < left; i += kBlock) q[i] = Act<DT>::st(Act<DT>::ld(p[i]) * f);
     }
 }
 
-// f(tensor, first element) over this workgroup's chunks
-template <typename F> __device__ __forceinline__ void over_chunks(const ClipArgs &a, F &&f)
+// f(tensor, first element, end) over this workgroup's runs
+template <typename F> __device__ __forceinline__ void over_runs(const ClipArgs &a, F &&f)
 {
     uint32_t c = (uint32_t)((uint64_t)a.chunks * blockIdx.x / gridDim.x);
     const uint32_t end = (uint32_t)((uint64_t)a.chunks * (blockIdx.x + 1) / gridDim.x);
     if (c >= end) return;
-    int lo = 0, hi = a.count - 1;  // the last tensor that starts at or before chunk c
-    while (lo < hi) {
-        const int mid = (lo + hi + 1) >> 1;
-        if (a.first[mid] <= c) lo = mid;
+    int t = 0, hi = a.count - 1;  // the last tensor that starts at or before chunk c
+    while (t < hi) {
+        const int mid = (t + hi + 1) >> 1;
+        if (a.first[mid] <= c) t = mid;
         else hi = mid - 1;
     }
-    for (; c < end; ++c) {
-        while (lo + 1 < a.count && a.first[lo + 1] <= c) ++lo;
-        f(lo, (int64_t)(c - a.first[lo]) * kChunk);
+    for (; c < end; ++t) {
+        const uint32_t first = a.first[t], stop = t + 1 < a.count && a.first[t + 1] < end ? a.first[t + 1] : end;
+        const int64_t to = (int64_t)(stop - first) * kChunk;
+        f(t, (int64_t)(c - first) * kChunk, to < a.n[t] ? to : a.n[t]);
+        c = stop;
     }
 }
 
@@ -147,10 +181,10 @@ template <int NORM> __global__ __launch_bounds__(kBlock) void k_grad_norm(const 
 {
     double sum = 0.0;
     uint32_t top = 0;
-    over_chunks(a, [&](int t, int64_t start) {
-        if (a.dtype[t] == STACR_DTYPE_F32) chunk_norm<STACR_DTYPE_F32, NORM>(a.in[t], a.n[t], start, sum, top);
-        else if (a.dtype[t] == STACR_DTYPE_BF16) chunk_norm<STACR_DTYPE_BF16, NORM>(a.in[t], a.n[t], start, sum, top);
-        else chunk_norm<STACR_DTYPE_F16, NORM>(a.in[t], a.n[t], start, sum, top);
+    over_runs(a, [&](int t, int64_t from, int64_t to) {
+        if (a.dtype[t] == STACR_DTYPE_F32) run_norm<STACR_DTYPE_F32, NORM>(a.in[t], from, to, sum, top);
+        else if (a.dtype[t] == STACR_DTYPE_BF16) run_norm<STACR_DTYPE_BF16, NORM>(a.in[t], from, to, sum, top);
+        else run_norm<STACR_DTYPE_F16, NORM>(a.in[t], from, to, sum, top);
     });
     const double v = block_join<NORM>(NORM == 0 ? (double)__uint_as_float(top) : sum);
     if (threadIdx.x == 0) a.part[blockIdx.x] = v;
@@ -159,6 +193,7 @@ template <int NORM> __global__ __launch_bounds__(kBlock) void k_grad_norm(const 
 template <int NORM> __global__ __launch_bounds__(kBlock) void k_grad_clip(const ClipArgs a)
 {
     double v = 0.0;
+#pragma unroll 8
     for (int i = threadIdx.x; i < a.parts; i += kBlock) v = joined<NORM>(v, a.part[i]);
     v = block_join<NORM>(v);
     const double norm = NORM == 2 ? sqrt(v) : v;
@@ -168,11 +203,11 @@ template <int NORM> __global__ __launch_bounds__(kBlock) void k_grad_clip(const 
     double f = a.max_norm / (norm + a.eps);
     if (f > 1.0) f = 1.0;
     const float factor = (float)f;
-    over_chunks(a, [&](int t, int64_t start) {
+    over_runs(a, [&](int t, int64_t from, int64_t to) {
         if (factor == 1.0f && a.in[t] == a.out[t]) return;
-        if (a.dtype[t] == STACR_DTYPE_F32) chunk_scale<STACR_DTYPE_F32>(a.in[t], a.out[t], a.n[t], start, factor);
-        else if (a.dtype[t] == STACR_DTYPE_BF16) chunk_scale<STACR_DTYPE_BF16>(a.in[t], a.out[t], a.n[t], start, factor);
-        else chunk_scale<STACR_DTYPE_F16>(a.in[t], a.out[t], a.n[t], start, factor);
+        if (a.dtype[t] == STACR_DTYPE_F32) run_scale<STACR_DTYPE_F32>(a.in[t], a.out[t], from, to, factor);
+        else if (a.dtype[t] == STACR_DTYPE_BF16) run_scale<STACR_DTYPE_BF16>(a.in[t], a.out[t], from, to, factor);
+        else run_scale<STACR_DTYPE_F16>(a.in[t], a.out[t], from, to, factor);
     });
 }
 
@@ -228,7 +263,7 @@ int stacr_clip_gradients(int count, const void *const *in, void *const *out, con
             a.in[a.count] = in[i];
             a.out[a.count] = out ? out[i] : nullptr;
             a.n[a.count] = sizes[i];
-            a.dtype[a.count] = (uint8_t)dtypes[i];
+            a.dtype[a.count] = (uint32_t)dtypes[i];
             a.first[a.count++] = a.chunks;
             a.chunks += (uint32_t)chunks_of(sizes[i]);
         }
@@ -238,7 +273,6 @@ int stacr_clip_gradients(int count, const void *const *in, void *const *out, con
         return (int)hmax<int64_t>(1, hmin<int64_t>(a.chunks, (int64_t)kGroups * a.chunks / hmax<int64_t>(1, total)));
     };
     ClipArgs a{};
-    a.norm = norm_type;
     a.max_norm = max_norm;
     a.eps = eps;
     int parts = 0;

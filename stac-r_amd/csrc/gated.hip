@@ -38,15 +38,15 @@ struct MmArgs {
     int64_t M, N, K;                 // N: columns of C (of one half of it, for the gated products)
     int64_t a_half;                  // second half of C's rows: A's column offset
     int halves;
-    int mt, nt, splits;
+    int mt, nt, splits, tiles;       // tiles: of all halves and splits
     void *out, *out2;
     int64_t ldo;
     int out_dt;
-    bool vec;                        // rows of out (and dh) are whole, aligned 16-byte pieces
     float *part;                     // splits > 1: fp32 partial products [split][half][M][N]
     // gated epilogues
     const void *bias_g, *bias_u, *dh;
-    void *gate, *up;                 // kept pre-activations or NULL
+    void *gate, *up;                 // kept pre-activations or NULL, in the type, or with the low
+    uint8_t *gate_low, *up_low;      // bytes not NULL the upper 16 of 24 bits
     uint16_t *dgu;                   // [plane][M][2 * ff_pad]
     int64_t ff_pad, plane;
     int act;
@@ -126,185 +126,154 @@ __device__ __forceinline__ void split_f32(float v, uint16_t (&p)[kPlanes])
     p[2] = (uint16_t)(__float_as_uint(r1 - __uint_as_float(mid)) >> 16);
 }
 
-// four consecutive values of a row of type DT (n .. n + 3, those below N)
-template <int DT>
-__device__ __forceinline__ void store4(void *out, int64_t row, int64_t n, int64_t N, const float (&v)[4], bool vec)
+// The 24-bit form of a kept pre-activation: fp32 rounded to its upper three bytes (2^-16 relative).  Kept in
+// the 16-bit type, g and u would each put another rounding of that type into dg and du; this one is a
+// hundredth of it.
+__device__ __forceinline__ uint32_t to_24(float v)
+{
+    return v != v ? 0x7fc00000u : __float_as_uint(v) + 0x80u;  // the lowest byte is not kept
+}
+
+// ------------------------------------------------------------------ rows of a result
+// Eight consecutive values at column n of a row at p: whole where all are below N, at any alignment.
+// (Stores of 16 bytes a lane, 64 neighbouring bytes from four lanes.)
+__device__ __forceinline__ void put8(uint16_t *p, uint4 v, int64_t n, int64_t N)
+{
+    if (n + 8 <= N) {
+        __builtin_memcpy(p + n, &v, 16);
+    } else {
+        const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+        for (int k = 0; k < 8; ++k)
+            if (n + k < N) p[n + k] = (uint16_t)(w[k >> 1] >> (k & 1) * 16);
+    }
+}
+
+__device__ __forceinline__ void put4f(float *p, const float (&v)[4], int64_t n, int64_t N)
+{
+    if (n + 4 <= N) {
+        __builtin_memcpy(p + n, v, 16);
+    } else {
+#pragma unroll
+        for (int k = 0; k < 4; ++k)
+            if (n + k < N) p[n + k] = v[k];
+    }
+}
+
+template <typename T> __device__ __forceinline__ uint4 get8(const T *p, int64_t n, int64_t N)
+{
+    uint4 v = make_uint4(0, 0, 0, 0);
+    if (n + 8 <= N) {
+        __builtin_memcpy(&v, p + n, 16);
+    } else {
+        uint32_t w[4] = {};
+#pragma unroll
+        for (int k = 0; k < 8; ++k)
+            if (n + k < N) w[k >> 1] |= (uint32_t)p[n + k] << (k & 1) * 16;
+        v = make_uint4(w[0], w[1], w[2], w[3]);
+    }
+    return v;
+}
+
+template <int DT> __device__ __forceinline__ uint2 pack4(const float (&v)[4])
 {
     using A = Act<DT>;
-    typename A::T *p = static_cast<typename A::T *>(out) + row + n;
-    if (vec && n + 3 < N) {
-        if constexpr (DT == STACR_DTYPE_F32) {
-            *reinterpret_cast<float4 *>(p) = make_float4(v[0], v[1], v[2], v[3]);
-        } else {
-            *reinterpret_cast<uint2 *>(p) = make_uint2((uint32_t)A::st(v[0]) | (uint32_t)A::st(v[1]) << 16,
-                                                       (uint32_t)A::st(v[2]) | (uint32_t)A::st(v[3]) << 16);
+    return make_uint2((uint32_t)A::st(v[0]) | (uint32_t)A::st(v[1]) << 16, (uint32_t)A::st(v[2]) | (uint32_t)A::st(v[3]) << 16);
+}
+
+__device__ __forceinline__ uint4 eights(uint2 a, uint2 b)
+{
+    mm_eights(a.x, b.x);
+    mm_eights(a.y, b.y);
+    return make_uint4(a.x, a.y, b.x, b.y);
+}
+
+// Quads of the neighbouring 16-column blocks a, b of this lane's row, to columns n .. + 31 (below N) of the
+// row at p; `in`: the row is there
+template <int DT>
+__device__ __forceinline__ void put_blocks(void *p, int lane, const float (&a)[4], const float (&b)[4], int64_t n, int64_t N,
+                                           bool in)
+{
+    if constexpr (DT == STACR_DTYPE_F32) {
+        if (!in) return;
+        put4f(static_cast<float *>(p), a, n + (lane >> 4) * 4, N);
+        put4f(static_cast<float *>(p), b, n + 16 + (lane >> 4) * 4, N);
+    } else {
+        const uint4 v = eights(pack4<DT>(a), pack4<DT>(b));  // every lane takes part
+        if (in) put8(static_cast<uint16_t *>(p), v, n + (lane >> 4) * 8, N);
+    }
+}
+
+// dg or du of the same into a row of [dg | du] (fp32: of its four planes)
+template <int DT>
+__device__ __forceinline__ void put_slopes(uint16_t *p, int64_t plane, int lane, const float (&a)[4], const float (&b)[4],
+                                           int64_t n, int64_t N, bool in)
+{
+    if constexpr (DT == STACR_DTYPE_F32) {
+        uint16_t s[8][kPlanes];
+#pragma unroll
+        for (int r = 0; r < 4; ++r) split_f32(a[r], s[r]), split_f32(b[r], s[4 + r]);
+#pragma unroll
+        for (int t = 0; t < kPlanes; ++t) {
+            const uint2 x = make_uint2((uint32_t)s[0][t] | (uint32_t)s[1][t] << 16, (uint32_t)s[2][t] | (uint32_t)s[3][t] << 16);
+            const uint2 y = make_uint2((uint32_t)s[4][t] | (uint32_t)s[5][t] << 16, (uint32_t)s[6][t] | (uint32_t)s[7][t] << 16);
+            const uint4 v = eights(x, y);
+            if (in) put8(p + t * plane, v, n + (lane >> 4) * 8, N);
         }
+    } else {
+        put_blocks<DT>(p, lane, a, b, n, N, in);
+    }
+}
+
+// the kept pre-activations of the same: in the type, or the upper 16 of 24 bits and the low byte
+template <int DT>
+__device__ __forceinline__ void put_kept(void *p, uint8_t *low, int64_t at, int lane, const float (&a)[4], const float (&b)[4],
+                                         int64_t n, int64_t N, bool in)
+{
+    if (DT == STACR_DTYPE_F32 || !low) {
+        put_blocks<DT>(static_cast<typename Act<DT>::T *>(p) + at, lane, a, b, n, N, in);
         return;
     }
+    uint32_t x[4], y[4];
 #pragma unroll
-    for (int r = 0; r < 4; ++r)
-        if (n + r < N) p[r] = A::st(v[r]);
-}
-
-template <int DT>
-__device__ __forceinline__ void load4(const void *in, int64_t row, int64_t n, int64_t N, float (&v)[4], bool vec)
-{
-    using A = Act<DT>;
-    const typename A::T *p = static_cast<const typename A::T *>(in) + row + n;
-    if (vec && n + 3 < N) {
-        if constexpr (DT == STACR_DTYPE_F32) {
-            const float4 w = *reinterpret_cast<const float4 *>(p);
-            v[0] = w.x; v[1] = w.y; v[2] = w.z; v[3] = w.w;
-        } else {
-            const uint2 w = *reinterpret_cast<const uint2 *>(p);
-            v[0] = A::ld((typename A::T)(w.x & 0xffffu)); v[1] = A::ld((typename A::T)(w.x >> 16));
-            v[2] = A::ld((typename A::T)(w.y & 0xffffu)); v[3] = A::ld((typename A::T)(w.y >> 16));
-        }
-        return;
-    }
+    for (int r = 0; r < 4; ++r) x[r] = to_24(a[r]), y[r] = to_24(b[r]);
+    const uint4 v = eights(make_uint2(x[0] >> 16 | (x[1] & 0xffff0000u), x[2] >> 16 | (x[3] & 0xffff0000u)),
+                           make_uint2(y[0] >> 16 | (y[1] & 0xffff0000u), y[2] >> 16 | (y[3] & 0xffff0000u)));
+    uint32_t lx = 0, ly = 0;
 #pragma unroll
-    for (int r = 0; r < 4; ++r) v[r] = n + r < N ? A::ld(p[r]) : 0.0f;
-}
-
-// dg and du of four outputs f .. f + 3 of token m into [dg | du] (fp32: its four planes)
-template <int DT>
-__device__ __forceinline__ void store_dgu(uint16_t *dgu, int64_t ff_pad, int64_t plane, int64_t m, int64_t f,
-                                          const float (&dg)[4], const float (&du)[4])
-{
-    uint16_t *p = dgu + m * 2 * ff_pad + f;
+    for (int r = 0; r < 4; ++r) lx |= (x[r] >> 8 & 255u) << r * 8, ly |= (y[r] >> 8 & 255u) << r * 8;
+    mm_eights(lx, ly);
+    if (!in) return;
+    n += (lane >> 4) * 8;
+    put8(static_cast<uint16_t *>(p) + at, v, n, N);
+    uint8_t *q = low + at + n;
+    if (n + 8 <= N) {
+        const uint2 w = make_uint2(lx, ly);
+        __builtin_memcpy(q, &w, 8);
+    } else {
 #pragma unroll
-    for (int half = 0; half < 2; ++half) {
-        const float(&v)[4] = half ? du : dg;
-        uint16_t *q = p + half * ff_pad;
-        if constexpr (DT == STACR_DTYPE_F32) {
-            uint16_t s[4][kPlanes];
-#pragma unroll
-            for (int r = 0; r < 4; ++r) split_f32(v[r], s[r]);
-#pragma unroll
-            for (int t = 0; t < kPlanes; ++t)
-                *reinterpret_cast<uint2 *>(q + t * plane) =
-                    make_uint2((uint32_t)s[0][t] | (uint32_t)s[1][t] << 16, (uint32_t)s[2][t] | (uint32_t)s[3][t] << 16);
-        } else {
-            using A = Act<DT>;
-            *reinterpret_cast<uint2 *>(q) = make_uint2((uint32_t)A::st(v[0]) | (uint32_t)A::st(v[1]) << 16,
-                                                       (uint32_t)A::st(v[2]) | (uint32_t)A::st(v[3]) << 16);
-        }
+        for (int k = 0; k < 8; ++k)
+            if (n + k < N) q[k] = (uint8_t)((k < 4 ? lx : ly) >> (k & 3) * 8);
     }
 }
 
-// A workgroup's results on their way out: rows of COLS values of type DT in LDS (16 bytes between rows
-// against bank conflicts), then whole 16-byte pieces of rows to memory, consecutive lanes consecutive.
-template <int DT, int COLS> struct Staged {
-    using T = typename Act<DT>::T;
-    static constexpr int kVec = 16 / sizeof(T), kPieces = COLS / kVec;
-    static constexpr uint32_t pitch = COLS * sizeof(T) + 16;
-
-    static __device__ __forceinline__ void put4(unsigned char *lds, int row, int col, const float (&v)[4])
-    {
-        using A = Act<DT>;
-        unsigned char *p = lds + row * pitch + col * sizeof(T);
-        if constexpr (DT == STACR_DTYPE_F32) *reinterpret_cast<float4 *>(p) = make_float4(v[0], v[1], v[2], v[3]);
-        else
-            *reinterpret_cast<uint2 *>(p) = make_uint2((uint32_t)A::st(v[0]) | (uint32_t)A::st(v[1]) << 16,
-                                                       (uint32_t)A::st(v[2]) | (uint32_t)A::st(v[3]) << 16);
-    }
-
-    static __device__ __forceinline__ void get4(const unsigned char *lds, int row, int col, float (&v)[4])
-    {
-        load4<DT>(lds + row * pitch, 0, col, COLS, v, true);
-    }
-
-    // rows m0 .. of `out` (those below M), columns n0 .. (below N)
-    static __device__ __forceinline__ void store(const unsigned char *lds, int rows, int threads, void *out, int64_t ldo,
-                                                 int64_t m0, int64_t M, int64_t n0, int64_t N, bool vec)
-    {
-        const int live = (int)(M - m0 < rows ? M - m0 : rows);
-        T *base = static_cast<T *>(out) + m0 * ldo + n0;
-        const int cols = (int)(N - n0 < COLS ? N - n0 : COLS);
-        for (int i = threadIdx.x; i < live * kPieces; i += threads) {
-            const int r = i / kPieces, c = (i % kPieces) * kVec;
-            const uint4 v = *reinterpret_cast<const uint4 *>(lds + r * pitch + c * sizeof(T));
-            T *p = base + r * ldo + c;
-            if (vec && c + kVec <= cols) {
-                *reinterpret_cast<uint4 *>(p) = v;
-            } else {
-                const T *e = reinterpret_cast<const T *>(lds + r * pitch) + c;
-                for (int k = 0; k < kVec; ++k)
-                    if (c + k < cols) p[k] = e[k];
-            }
-        }
-    }
-
-    // the same rows and columns of `in` into LDS, zeros outside
-    static __device__ __forceinline__ void load(unsigned char *lds, int rows, int threads, const void *in, int64_t ld,
-                                                int64_t m0, int64_t M, int64_t n0, int64_t N, bool vec)
-    {
-        const int live = (int)(M - m0 < rows ? M - m0 : rows);
-        const T *base = static_cast<const T *>(in) + m0 * ld + n0;
-        const int cols = (int)(N - n0 < COLS ? N - n0 : COLS);
-#pragma unroll 4
-        for (int i = threadIdx.x; i < rows * kPieces; i += threads) {
-            const int r = i / kPieces, c = (i % kPieces) * kVec;
-            uint4 v = make_uint4(0, 0, 0, 0);
-            if (r < live) {
-                const T *p = base + r * ld + c;
-                if (vec && c + kVec <= cols) {
-                    v = *reinterpret_cast<const uint4 *>(p);
-                } else {
-                    T e[kVec];
-                    for (int k = 0; k < kVec; ++k) e[k] = c + k < cols ? p[k] : T(0);
-                    __builtin_memcpy(&v, e, 16);
-                }
-            }
-            *reinterpret_cast<uint4 *>(lds + r * pitch + c * sizeof(T)) = v;
-        }
-    }
-};
-
-// LDS of a product's workgroup: two stages, or what its epilogue stages
-template <int DT, int EPI, int BM, int BN> constexpr size_t mm_lds()
-{
-    const size_t stages = 2 * (BM + BN) * 128;
-    size_t out = 0;
-    if (EPI == kFwd) out = BM * Staged<DT, BN / 2>::pitch;
-    if (EPI == kBwd) out = BM * Staged<DT, BN / 2>::pitch * (DT == STACR_DTYPE_F32 ? 1 : 2);
-    if (EPI == kStore) out = BM * Staged<STACR_DTYPE_BF16, BN>::pitch;
-    return out > stages ? out : stages;
-}
-
-// A workgroup's tile: consecutive logical ids share an XCD (ids are dealt to the 8 XCDs round-robin)
-// and walk `kGroup` tile rows together, so that an XCD's tiles share operands in its L2.
+// A workgroup takes every gridDim.x-th tile.  Consecutive logical tiles share an XCD (workgroups are dealt
+// to the 8 XCDs round-robin, and gridDim.x is a multiple of 8 where there is more than one round) and
+// walk `kGroup` tile rows together, so that an XCD's tiles share operands in its L2.
 constexpr int kGroup = 8;
 
 template <int DT, bool AK, bool BK, int EPI, int BM, int BN, int WM, int WN>
-__global__ __launch_bounds__(WM *WN * 64) void k_gated_mm(const MmArgs p)
+__global__ __launch_bounds__(WM *WN * 64, 1) void k_gated_mm(const MmArgs p)
 {
     constexpr int MT = DT == STACR_DTYPE_F16 ? STACR_DTYPE_F16 : STACR_DTYPE_BF16;  // the operands' type
     constexpr int NW = WM * WN, TM = BM / WM, TN = BN / WN, MI = TM / 16, NI = TN / 16;
     constexpr uint32_t kA = BM * 128, kStage = (BM + BN) * 128;
     constexpr bool DUAL = EPI != kStore;
+    static_assert(NI % 4 == 0, "results leave in eights of two blocks (of two pairs)");
     extern __shared__ __attribute__((aligned(1024))) unsigned char lds[];
     const int lane = threadIdx.x & 63;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int wm = wave / WN, wn = wave % WN;
-
-    // tile
-    const int total = gridDim.x;
-    int id = blockIdx.x;
-    {
-        const int q = total >> 3, r = total & 7, x = id & 7;
-        id = x * q + (x < r ? x : r) + (id >> 3);
-    }
-    const int split = id / (p.mt * p.nt * p.halves);
-    id -= split * p.mt * p.nt * p.halves;
-    const int mrows = p.mt * p.halves;
-    const int group = id / (kGroup * p.nt), first = group * kGroup;
-    const int size = mrows - first < kGroup ? mrows - first : kGroup;
-    const int in = id - group * kGroup * p.nt;
-    const int mrow = first + in % size, ntile = in / size;
-    const int half = mrow / p.mt;
-    const int64_t m0 = (int64_t)(mrow - half * p.mt) * BM;
-    const int64_t n0 = (int64_t)ntile * (DUAL ? BN / 2 : BN);
 
     MmLoader<AK, BM, NW> la;
     MmLoader<BK, BN, NW> lb;
@@ -314,29 +283,53 @@ __global__ __launch_bounds__(WM *WN * 64) void k_gated_mm(const MmArgs p)
 #pragma unroll
         for (int i = 0; i < lb.kPer; ++i) {
             const int row = (wave * lb.kPer + i) * 8 + (lane >> 3);
-            lb.off[i] = (uint32_t)((row >> 5) * 16 + (row & 15)) * (uint32_t)p.b.ld * 2 + lb.kc * 2;
+            lb.off[i] = (uint32_t)((row >> 5) * 16 + (row & 15)) * (uint32_t)p.b.ld * 2 + lb.kc[i & 1] * 2;
         }
     }
     MmReader<AK, BM, MI> ra;
     MmReader<BK, BN, NI> rb;
     ra.init(lane, wm * TM);
     rb.init(lane, wn * TN);
-
     const int ksteps = (int)((p.K + kMmK - 1) / kMmK), steps = ksteps * p.nseg;
-    const int begin = (int)((int64_t)steps * split / p.splits), end = (int)((int64_t)steps * (split + 1) / p.splits);
 
-    // The step that is loaded next: bytes from the operands' first values of this tile in it to their end
-    // bound the reads (rows past the last, K past the last).
+    struct Tile {
+        int64_t m0, n0;
+        int half, split, begin, count;  // steps begin .. begin + count - 1
+    };
+    const auto locate = [&](int id) __attribute__((always_inline)) {
+        Tile t;
+        const int q = p.tiles >> 3, r = p.tiles & 7, x = id & 7;
+        id = x * q + (x < r ? x : r) + (id >> 3);
+        const int each = p.mt * p.nt * p.halves;
+        t.split = id / each;
+        id -= t.split * each;
+        const int mrows = p.mt * p.halves;
+        const int group = id / (kGroup * p.nt), first = group * kGroup;
+        const int size = mrows - first < kGroup ? mrows - first : kGroup;
+        const int in = id - group * kGroup * p.nt;
+        const int mrow = first + in % size;
+        t.half = mrow / p.mt;
+        t.m0 = (int64_t)(mrow - t.half * p.mt) * BM;
+        t.n0 = (int64_t)(in / size) * (DUAL ? BN / 2 : BN);
+        t.begin = (int)((int64_t)steps * t.split / p.splits);
+        t.count = (int)((int64_t)steps * (t.split + 1) / p.splits) - t.begin;
+        return t;
+    };
+
+    // The step that is loaded next, and its tile (one step ahead of the one that is multiplied): bytes from
+    // the operands' first values of this tile in it to their end bound the reads (rows past the last, K
+    // past the last).
     const unsigned char *pa = nullptr, *pb = nullptr, *pb2 = nullptr;
     int64_t left_a = 0, left_b = 0;
     const int64_t step_a = AK ? kMmK * 2 : p.a.ld * (kMmK * 2), step_b = BK ? kMmK * 2 : p.b.ld * (kMmK * 2);
-    int seg = 0, ks = 0;
-    auto seek = [&](int s, int k) {
+    int ahead = blockIdx.x, seg = 0, ks = 0, todo = 0;
+    Tile lt{};
+    const auto seek = [&](int s, int k) __attribute__((always_inline)) {
         seg = s;
         ks = k;
         const int64_t k0 = (int64_t)k * kMmK, kpad = (p.K + 7) & ~7ll;
-        const int64_t at_a = AK ? m0 * p.a.ld + k0 : k0 * p.a.ld + m0 + half * p.a_half;
-        const int64_t at_b = BK ? n0 * p.b.ld + k0 : k0 * p.b.ld + n0;
+        const int64_t at_a = AK ? lt.m0 * p.a.ld + k0 : k0 * p.a.ld + lt.m0 + lt.half * p.a_half;
+        const int64_t at_b = BK ? lt.n0 * p.b.ld + k0 : k0 * p.b.ld + lt.n0;
         const int64_t end_a = AK ? (p.a.extent - 1) * p.a.ld + kpad : (p.K - 1) * p.a.ld + p.a.extent;
         const int64_t end_b = BK ? (p.b.extent - 1) * p.b.ld + kpad : (p.K - 1) * p.b.ld + p.b.extent;
         pa = reinterpret_cast<const unsigned char *>(p.a.seg[s] + at_a);
@@ -345,192 +338,215 @@ __global__ __launch_bounds__(WM *WN * 64) void k_gated_mm(const MmArgs p)
         left_a = (end_a - at_a) * 2;
         left_b = (end_b - at_b) * 2;
     };
-    auto next = [&] {
-        if (++ks == ksteps) {
-            if (seg + 1 < p.nseg) seek(seg + 1, 0);
+    const auto open = [&]() __attribute__((always_inline)) {
+        lt = locate(ahead);
+        todo = lt.count;
+        seek(lt.begin / ksteps, lt.begin % ksteps);
+    };
+    const auto next = [&]() __attribute__((always_inline)) {
+        if (--todo > 0) {
+            if (++ks < ksteps) {
+                pa += step_a;
+                pb += step_b;
+                if constexpr (DUAL) pb2 += step_b;
+                left_a -= step_a;
+                left_b -= step_b;
+            } else {
+                seek(seg + 1, 0);
+            }
+        } else if ((ahead += gridDim.x) < p.tiles) {
+            open();
         } else {
-            pa += step_a;
-            pb += step_b;
-            if constexpr (DUAL) pb2 += step_b;
-            left_a -= step_a;
-            left_b -= step_b;
+            left_a = left_b = 0;  // nothing more: zeros
+            todo = 1;
         }
     };
-    auto load = [&](unsigned char *__restrict__ at) {
+    const auto load = [&](unsigned char *at) __attribute__((always_inline)) {
         const uint32_t k = (uint32_t)ks * kMmK;
-        {
-            const auto r = mm_rsrc(pa, left_a);
-            const bool live = !AK || k + la.kc < (uint32_t)p.K;
+        const auto r = mm_rsrc(pa, left_a);
 #pragma unroll
-            for (int i = 0; i < la.kPer; ++i) mm_copy16(r, at + (wave * la.kPer + i) * 1024, live ? la.off[i] : kMmPast);
-        }
-        const bool live = !BK || k + lb.kc < (uint32_t)p.K;
-        const auto r = mm_rsrc(pb, left_b), r2 = mm_rsrc(pb2, left_b);
+        for (int i = 0; i < la.kPer; ++i)
+            mm_copy16(r, at + (wave * la.kPer + i) * 1024, !AK || k + la.kc[i & 1] < (uint32_t)p.K ? la.off[i] : kMmPast);
+        const auto s = mm_rsrc(pb, left_b), s2 = mm_rsrc(pb2, left_b);
 #pragma unroll
         for (int i = 0; i < lb.kPer; ++i) {
             const bool second = DUAL && ((wave * lb.kPer + i) & 2);  // 8 rows of one copy are of one weight
-            mm_copy16(second ? r2 : r, at + kA + (wave * lb.kPer + i) * 1024, live ? lb.off[i] : kMmPast);
+            mm_copy16(second ? s2 : s, at + kA + (wave * lb.kPer + i) * 1024,
+                      !BK || k + lb.kc[i & 1] < (uint32_t)p.K ? lb.off[i] : kMmPast);
         }
     };
 
     mmf4 acc[MI][NI];
-#pragma unroll
-    for (int i = 0; i < MI; ++i)
-#pragma unroll
-        for (int j = 0; j < NI; ++j) acc[i][j] = mmf4{0.0f, 0.0f, 0.0f, 0.0f};
-
     // One step: the next one's copies into `to`, the products of what is in `from`.  Two pointers that do
     // not alias: without that knowledge the compiler waits for the copies before it reads.
-    auto step = [&](const unsigned char *__restrict__ from, unsigned char *__restrict__ to, bool more) {
-        if (more) load(to);
-        const unsigned char *ta = from, *tb = from + kA;
+    const auto step = [&](const unsigned char *__restrict__ from, unsigned char *__restrict__ to) {
+        load(to);
+        __builtin_amdgcn_sched_barrier(0);  // all copies first: among the reads they come late
 #pragma unroll
         for (int kk = 0; kk < 2; ++kk) {
             uint4 av[MI], bv[NI];
 #pragma unroll
-            for (int j = 0; j < NI; ++j) bv[j] = rb.get(tb, j, kk, lane);
+            for (int j = 0; j < NI; ++j) bv[j] = rb.get(from + kA, j, kk, lane);
 #pragma unroll
-            for (int i = 0; i < MI; ++i) av[i] = ra.get(ta, i, kk, lane);
+            for (int i = 0; i < MI; ++i) av[i] = ra.get(from, i, kk, lane);
 #pragma unroll
             for (int i = 0; i < MI; ++i)
 #pragma unroll
                 for (int j = 0; j < NI; ++j) acc[i][j] = mm_mfma<MT>(bv[j], av[i], acc[i][j]);
         }
+        // Reads run two rows of blocks ahead of their products.  (Not where both operands come in halves and two
+        // workgroups share a CU: there the compiler's own order was 12 % faster, everywhere else 5 to 12 % slower.)
+        if constexpr (AK || BK || MI > 4) {
+            constexpr int ra_n = AK ? 1 : 2, rb_n = BK ? 1 : 2;
+            constexpr int kAll = 2 * (MI * ra_n + NI * rb_n), kFirst = NI * rb_n + 2 * ra_n;
+            constexpr int kEach = (kAll - kFirst + 2 * MI - 4) / (2 * MI - 3);
+            __builtin_amdgcn_sched_group_barrier(0x100, kFirst, 0);
+#pragma unroll
+            for (int i = 0; i < 2 * MI; ++i) {
+                __builtin_amdgcn_sched_group_barrier(0x008, NI, 0);
+                __builtin_amdgcn_sched_group_barrier(0x100, kEach, 0);
+            }
+        }
     };
-    if (begin < end) {
-        seek(begin / ksteps, begin % ksteps);
-        load(lds);
-        next();
-    }
-    for (int it = begin; it < end; ++it) {
-        const int buf = (it - begin) & 1;
-        __builtin_amdgcn_s_waitcnt(0x0070);  // vmcnt(0) lgkmcnt(0): this wave's copies of this step are in LDS
-        asm volatile("s_barrier" ::: "memory");  // and everybody's; the other stage has been read
-        step(lds + buf * kStage, lds + (buf ^ 1) * kStage, it + 1 < end);
-        next();
-    }
 
-    // a lane holds, of each 16 x 16 block, columns 4 (lane / 16) .. + 3 of row lane % 16
-    constexpr int NT = NW * 64;
-    const int row0 = wm * TM + (lane & 15), quad = (lane >> 4) * 4;
-    __syncthreads();  // the last step has been read
-    if constexpr (EPI == kStore) {
-        void *o = half ? p.out2 : p.out;
-        if (p.splits > 1 || p.out_dt == STACR_DTYPE_F32) {
-            float *out = p.splits > 1 ? p.part + ((int64_t)split * p.halves + half) * p.M * p.N : static_cast<float *>(o);
-            const bool vec = p.splits > 1 ? (p.N & 3) == 0 : p.vec;
+    open();
+    load(lds);
+    int buf = 0;
+    for (int id = blockIdx.x; id < p.tiles; id += gridDim.x) {
+        const Tile t = lt;  // the loader enters the next tile with this one's last step
+#pragma unroll
+        for (int i = 0; i < MI; ++i)
+#pragma unroll
+            for (int j = 0; j < NI; ++j) acc[i][j] = mmf4{0.0f, 0.0f, 0.0f, 0.0f};
+        for (int it = 0; it < t.count; ++it) {
+            next();
+            __builtin_amdgcn_s_waitcnt(0x0070);  // vmcnt(0) lgkmcnt(0): this wave's copies of this step are in LDS
+            asm volatile("s_barrier" ::: "memory");  // and everybody's; the other stage has been read
+            step(lds + buf * kStage, lds + (buf ^ 1) * kStage);
+            buf ^= 1;
+        }
+
+        // a lane holds, of each 16 x 16 block, columns 4 (lane / 16) .. + 3 of row lane % 16
+        const int64_t mfirst = t.m0 + wm * TM + (lane & 15);
+        const auto quad = [&](const mmf4 &w, float(&v)[4]) __attribute__((always_inline)) {
+#pragma unroll
+            for (int r = 0; r < 4; ++r) v[r] = w[r];
+        };
+        if constexpr (EPI == kStore) {
+            void *o = t.half ? p.out2 : p.out;
+            const bool wide = p.splits > 1 || p.out_dt == STACR_DTYPE_F32;
+            if (p.splits > 1) o = p.part + ((int64_t)t.split * p.halves + t.half) * p.M * p.N;
 #pragma unroll
             for (int i = 0; i < MI; ++i) {
-                const int64_t m = m0 + row0 + i * 16;
-                if (m >= p.M) continue;
+                const int64_t m = mfirst + i * 16;
 #pragma unroll
-                for (int j = 0; j < NI; ++j) {
-                    const float v[4] = {acc[i][j][0], acc[i][j][1], acc[i][j][2], acc[i][j][3]};
-                    store4<STACR_DTYPE_F32>(out, m * p.N, n0 + wn * TN + j * 16 + quad, p.N, v, vec);
+                for (int j = 0; j < NI; j += 2) {
+                    const int64_t n = t.n0 + wn * TN + j * 16;
+                    float a[4], b[4];
+                    quad(acc[i][j], a);
+                    quad(acc[i][j + 1], b);
+                    if (wide) put_blocks<STACR_DTYPE_F32>(static_cast<float *>(o) + m * p.N, lane, a, b, n, p.N, m < p.M);
+                    else put_blocks<MT>(static_cast<uint16_t *>(o) + m * p.N, lane, a, b, n, p.N, m < p.M);
                 }
             }
         } else {
-            using S = Staged<MT, BN>;
+            constexpr bool EXACT = DT == STACR_DTYPE_F32;
+            using T = typename Act<DT>::T;
+            const int64_t f0 = t.n0 + wn * (TN / 2);  // blocks (0, 1) of NI: gate and up of 16 outputs from f0 on
+            if (p.bias_g || p.bias_u) {
 #pragma unroll
-            for (int i = 0; i < MI; ++i)
+                for (int j = 0; j < NI; j += 2)
 #pragma unroll
-                for (int j = 0; j < NI; ++j) {
-                    const float v[4] = {acc[i][j][0], acc[i][j][1], acc[i][j][2], acc[i][j][3]};
-                    S::put4(lds, row0 + i * 16, wn * TN + j * 16 + quad, v);
-                }
-            __syncthreads();
-            S::store(lds, BM, NT, o, p.ldo, m0, p.M, n0, p.N, p.vec);
-        }
-    } else {
-        constexpr bool EXACT = DT == STACR_DTYPE_F32;
-        constexpr int F = BN / 2;
-        using S = Staged<DT, F>;
-        const int col0 = wn * (TN / 2) + quad;
-        if (p.bias_g || p.bias_u) {
+                    for (int r = 0; r < 4; ++r) {
+                        const int64_t f = f0 + j * 8 + (lane >> 4) * 4 + r;
+                        const float bg = p.bias_g && f < p.N ? load_any(p.bias_g, DT, f) : 0.0f;
+                        const float bu = p.bias_u && f < p.N ? load_any(p.bias_u, DT, f) : 0.0f;
 #pragma unroll
-            for (int j = 0; j < NI; j += 2) {
-                float bg[4] = {}, bu[4] = {};
-                if (p.bias_g) load4<DT>(p.bias_g, 0, n0 + col0 + j * 8, p.N, bg, false);
-                if (p.bias_u) load4<DT>(p.bias_u, 0, n0 + col0 + j * 8, p.N, bu, false);
-#pragma unroll
-                for (int i = 0; i < MI; ++i)
-#pragma unroll
-                    for (int r = 0; r < 4; ++r) acc[i][j][r] += bg[r], acc[i][j + 1][r] += bu[r];
-            }
-        }
-        if constexpr (EPI == kFwd) {
-            with_activation(p.act, [&](auto c) {
-#pragma unroll
-                for (int i = 0; i < MI; ++i)
-#pragma unroll
-                    for (int j = 0; j < NI; j += 2) {
-                        float h[4];
-#pragma unroll
-                        for (int r = 0; r < 4; ++r) {
-                            float a, slope;
-                            activate<EXACT, decltype(c)::value>(acc[i][j][r], a, slope);
-                            h[r] = a * acc[i][j + 1][r];
-                        }
-                        S::put4(lds, row0 + i * 16, col0 + j * 8, h);
+                        for (int i = 0; i < MI; ++i) acc[i][j][r] += bg, acc[i][j + 1][r] += bu;
                     }
-            });
-            __syncthreads();
-            S::store(lds, BM, NT, p.out, p.ldo, m0, p.M, n0, p.N, p.vec);
-            if (p.gate) {  // the kept pre-activations
-#pragma unroll
-                for (int which = 0; which < 2; ++which) {
-                    __syncthreads();
-#pragma unroll
-                    for (int i = 0; i < MI; ++i)
-#pragma unroll
-                        for (int j = 0; j < NI; j += 2) {
-                            const mmf4 &w = acc[i][j + which];
-                            const float v[4] = {w[0], w[1], w[2], w[3]};
-                            S::put4(lds, row0 + i * 16, col0 + j * 8, v);
-                        }
-                    __syncthreads();
-                    S::store(lds, BM, NT, which ? p.up : p.gate, p.ldo, m0, p.M, n0, p.N, p.vec);
-                }
             }
-        } else {
-            // dh is staged first; a lane's dg takes the place of the dh that it read, du a second stage
-            S::load(lds, BM, NT, p.dh, p.ldo, m0, p.M, n0, p.N, p.vec);
-            __syncthreads();
-            unsigned char *second = lds + BM * S::pitch;
-            with_activation(p.act, [&](auto c) {
+            if constexpr (EPI == kFwd) {
+                with_activation(p.act, [&](auto c) __attribute__((always_inline)) {
 #pragma unroll
-                for (int i = 0; i < MI; ++i) {
-                    __builtin_amdgcn_sched_barrier(0);  // a row of blocks at a time: all at once spill
-                    const int64_t m = m0 + row0 + i * 16;
+                    for (int i = 0; i < MI; ++i) {
+                        const int64_t m = mfirst + i * 16;
 #pragma unroll
-                    for (int j = 0; j < NI; j += 2) {
-                        float d[4], dg[4], du[4];
-                        S::get4(lds, row0 + i * 16, col0 + j * 8, d);
+                        for (int j = 0; j < NI; j += 4) {
+                            float h[2][4];
 #pragma unroll
-                        for (int r = 0; r < 4; ++r) {
-                            float a, slope;
-                            activate<EXACT, decltype(c)::value>(acc[i][j][r], a, slope);
-                            dg[r] = d[r] * acc[i][j + 1][r] * slope;
-                            du[r] = d[r] * a;
-                        }
-                        if constexpr (EXACT) {
-                            if (m < p.M && n0 + col0 + j * 8 < p.ff_pad)
-                                store_dgu<DT>(p.dgu, p.ff_pad, p.plane, m, n0 + col0 + j * 8, dg, du);
-                        } else {
-                            S::put4(lds, row0 + i * 16, col0 + j * 8, dg);
-                            S::put4(second, row0 + i * 16, col0 + j * 8, du);
+                            for (int b = 0; b < 2; ++b)
+#pragma unroll
+                                for (int r = 0; r < 4; ++r) {
+                                    float a, slope;
+                                    activate<EXACT, decltype(c)::value>(acc[i][j + 2 * b][r], a, slope);
+                                    h[b][r] = a * acc[i][j + 2 * b + 1][r];
+                                }
+                            put_blocks<DT>(static_cast<T *>(p.out) + m * p.ldo, lane, h[0], h[1], f0 + j * 8, p.N, m < p.M);
                         }
                     }
-                }
-            });
-            if constexpr (!EXACT) {
-                __syncthreads();
+                });
+                if (p.gate) {
 #pragma unroll
-                for (int which = 0; which < 2; ++which)
-                    S::store(which ? second : lds, BM, NT, p.dgu + which * p.ff_pad, 2 * p.ff_pad, m0, p.M, n0, p.ff_pad, true);
+                    for (int i = 0; i < MI; ++i) {
+                        const int64_t m = mfirst + i * 16;
+#pragma unroll
+                        for (int j = 0; j < NI; j += 4)
+#pragma unroll
+                            for (int u = 0; u < 2; ++u) {
+                                float a[4], b[4];
+                                quad(acc[i][j + u], a);
+                                quad(acc[i][j + 2 + u], b);
+                                put_kept<DT>(u ? p.up : p.gate, u ? p.up_low : p.gate_low, m * p.ldo, lane, a, b, f0 + j * 8,
+                                             p.N, m < p.M);
+                            }
+                    }
+                }
+            } else {
+                with_activation(p.act, [&](auto c) __attribute__((always_inline)) {
+#pragma unroll
+                    for (int i = 0; i < MI; ++i) {
+                        __builtin_amdgcn_sched_barrier(0);  // a row of blocks at a time: all at once spill
+                        const int64_t m = mfirst + i * 16;
+#pragma unroll
+                        for (int j = 0; j < NI; j += 4) {
+                            const int64_t f = f0 + j * 8;
+                            float d[2][4] = {}, dg[2][4], du[2][4];
+                            if constexpr (EXACT) {
+#pragma unroll
+                                for (int b = 0; b < 2; ++b)
+#pragma unroll
+                                    for (int r = 0; r < 4; ++r) {
+                                        const int64_t n = f + b * 16 + (lane >> 4) * 4 + r;
+                                        if (m < p.M && n < p.N) d[b][r] = static_cast<const float *>(p.dh)[m * p.ldo + n];
+                                    }
+                            } else {
+                                uint4 w = make_uint4(0, 0, 0, 0);
+                                if (m < p.M) w = get8(static_cast<const T *>(p.dh) + m * p.ldo, f + (lane >> 4) * 8, p.N);
+                                mm_quads(w.x, w.z);
+                                mm_quads(w.y, w.w);
+                                const uint32_t q[4] = {w.x, w.y, w.z, w.w};
+#pragma unroll
+                                for (int e = 0; e < 8; ++e) d[e >> 2][e & 3] = Act<DT>::ld((T)(q[e >> 1] >> (e & 1) * 16));
+                            }
+#pragma unroll
+                            for (int b = 0; b < 2; ++b)
+#pragma unroll
+                                for (int r = 0; r < 4; ++r) {
+                                    float a, slope;
+                                    activate<EXACT, decltype(c)::value>(acc[i][j + 2 * b][r], a, slope);
+                                    dg[b][r] = d[b][r] * acc[i][j + 2 * b + 1][r] * slope;
+                                    du[b][r] = d[b][r] * a;
+                                }
+                            uint16_t *row = p.dgu + m * 2 * p.ff_pad;
+                            put_slopes<DT>(row, p.plane, lane, dg[0], dg[1], f, p.ff_pad, m < p.M);
+                            put_slopes<DT>(row + p.ff_pad, p.plane, lane, du[0], du[1], f, p.ff_pad, m < p.M);
+                        }
+                    }
+                });
             }
         }
     }
+    __builtin_amdgcn_s_waitcnt(0x0070);  // the copies past the end
 }
 
 // sum of the partial products over the splits, in order, rounded once
@@ -587,48 +603,122 @@ __global__ __launch_bounds__(kBlock) void k_gated_pack(const void *__restrict__ 
 }
 
 // ------------------------------------------------------------------ kept pre-activations
-template <int DT>
+// [dg | du] from dh and the kept g and u, eight values a thread; LOW: g and u in 24 bits
+template <int DT, bool LOW>
 __global__ __launch_bounds__(kBlock) void k_gated_slopes(const void *__restrict__ dh, const void *__restrict__ gate,
-                                                         const void *__restrict__ up, int64_t rows, int64_t ff, int act,
-                                                         uint16_t *__restrict__ dgu, int64_t ff_pad, int64_t plane, bool vec)
+                                                         const void *__restrict__ up, const uint8_t *__restrict__ gate_low,
+                                                         const uint8_t *__restrict__ up_low, int64_t rows, int64_t ff, int act,
+                                                         uint16_t *__restrict__ dgu, int64_t ff_pad, int64_t plane)
 {
-    const int64_t quads = ff_pad / 4, n = rows * quads;
-    for (int64_t i = (int64_t)blockIdx.x * kBlock + threadIdx.x; i < n; i += (int64_t)gridDim.x * kBlock) {
-        const int64_t m = i / quads, f = (i - m * quads) * 4;
-        float d[4], g[4], u[4], dg[4], du[4];
-        load4<DT>(dh, m * ff, f, ff, d, vec);
-        load4<DT>(gate, m * ff, f, ff, g, vec);
-        load4<DT>(up, m * ff, f, ff, u, vec);
+    using T = typename Act<DT>::T;
+    constexpr bool EXACT = DT == STACR_DTYPE_F32;
+    const int64_t eighths = ff_pad / 8, n = rows * eighths;
+    with_activation(act, [&](auto c) __attribute__((always_inline)) {
+#pragma unroll 2
+        for (int64_t i = (int64_t)blockIdx.x * kBlock + threadIdx.x; i < n; i += (int64_t)gridDim.x * kBlock) {
+            const int64_t m = i / eighths, f = (i - m * eighths) * 8, at = m * ff + f;
+            const int have = ff - f < 8 ? (int)(ff - f) : 8;
+            const auto read = [&](const void *src, const uint8_t *low, float(&v)[8]) __attribute__((always_inline)) {
+                if constexpr (EXACT) {
+                    const float *p = static_cast<const float *>(src) + at;
+                    if (have == 8) {
+                        __builtin_memcpy(v, p, 32);
+                    } else {
 #pragma unroll
-        for (int r = 0; r < 4; ++r) {
-            float a, slope;
-            activate<DT == STACR_DTYPE_F32>(act, g[r], a, slope);
-            dg[r] = d[r] * u[r] * slope;
-            du[r] = d[r] * a;
+                        for (int k = 0; k < 8; ++k) v[k] = k < have ? p[k] : 0.0f;
+                    }
+                } else {
+                    const uint4 w = get8(static_cast<const T *>(src) + at, 0, have);
+                    const uint32_t q[4] = {w.x, w.y, w.z, w.w};
+                    uint2 b = make_uint2(0, 0);
+                    if (LOW && low) {
+                        if (have == 8) {
+                            __builtin_memcpy(&b, low + at, 8);
+                        } else {
+#pragma unroll
+                            for (int k = 0; k < 8; ++k)
+                                if (k < have) (k < 4 ? b.x : b.y) |= (uint32_t)low[at + k] << (k & 3) * 8;
+                        }
+                    }
+#pragma unroll
+                    for (int k = 0; k < 8; ++k) {
+                        const uint32_t h = q[k >> 1] >> (k & 1) * 16 & 0xffffu;
+                        if (LOW && low) v[k] = __uint_as_float(h << 16 | ((k < 4 ? b.x : b.y) >> (k & 3) * 8 & 255u) << 8);
+                        else v[k] = Act<DT>::ld((T)h);
+                    }
+                }
+            };
+            float d[8], g[8], u[8], dg[8], du[8];
+            read(dh, nullptr, d);
+            read(gate, gate_low, g);
+            read(up, up_low, u);
+#pragma unroll
+            for (int k = 0; k < 8; ++k) {
+                float a, slope;
+                activate<EXACT, decltype(c)::value>(g[k], a, slope);
+                dg[k] = d[k] * u[k] * slope;
+                du[k] = d[k] * a;
+            }
+            uint16_t *row = dgu + m * 2 * ff_pad + f;
+#pragma unroll
+            for (int half = 0; half < 2; ++half) {
+                const float(&v)[8] = half ? du : dg;
+                uint16_t *o = row + half * ff_pad;
+                if constexpr (EXACT) {
+                    uint16_t s[8][kPlanes];
+#pragma unroll
+                    for (int k = 0; k < 8; ++k) split_f32(v[k], s[k]);
+#pragma unroll
+                    for (int t = 0; t < kPlanes; ++t)
+                        *reinterpret_cast<uint4 *>(o + t * plane) =
+                            make_uint4((uint32_t)s[0][t] | (uint32_t)s[1][t] << 16, (uint32_t)s[2][t] | (uint32_t)s[3][t] << 16,
+                                       (uint32_t)s[4][t] | (uint32_t)s[5][t] << 16, (uint32_t)s[6][t] | (uint32_t)s[7][t] << 16);
+                } else {
+                    const float lo[4] = {v[0], v[1], v[2], v[3]}, hi[4] = {v[4], v[5], v[6], v[7]};
+                    const uint2 x = pack4<DT>(lo), y = pack4<DT>(hi);
+                    *reinterpret_cast<uint4 *>(o) = make_uint4(x.x, x.y, y.x, y.y);
+                }
+            }
         }
-        store_dgu<DT>(dgu, ff_pad, plane, m, f, dg, du);
-    }
+    });
 }
 
 // ------------------------------------------------------------------ bias gradients
-// column sums of [dg | du]: `parts` row ranges of partial sums, then their sum in order
+// column sums of [dg | du]: partial sums over row ranges of kBiasRows, then their sum in order.  A
+// workgroup takes 256 columns of a range: 32 threads of 8 columns, eight rows apart.
 constexpr int kBiasRows = 256;
 
 template <int DT>
 __global__ __launch_bounds__(kBlock) void k_gated_bias_part(const uint16_t *__restrict__ dgu, int64_t rows, int64_t ff_pad,
                                                             int64_t plane, float *__restrict__ part)
 {
-    const int64_t cols = 2 * ff_pad, c = (int64_t)blockIdx.x * kBlock + threadIdx.x;
-    if (c >= cols) return;
+    __shared__ float s[8][256 + 4];
+    constexpr int PL = DT == STACR_DTYPE_F32 ? 3 : 1;
+    const int64_t cols = 2 * ff_pad, c = (int64_t)blockIdx.x * 256 + (threadIdx.x & 31) * 8;
     const int64_t r0 = (int64_t)blockIdx.y * kBiasRows, r1 = r0 + kBiasRows < rows ? r0 + kBiasRows : rows;
-    float sum = 0.0f;
-    for (int64_t r = r0; r < r1; ++r) {
-        const uint16_t *p = dgu + r * cols + c;
-        if constexpr (DT == STACR_DTYPE_F32)
-            sum += bf16_bits_to_f(p[0]) + (bf16_bits_to_f(p[plane]) + bf16_bits_to_f(p[2 * plane]));
-        else sum += Act<DT>::ld(p[0]);
+    float sum[8] = {};
+    if (c < cols) {
+#pragma unroll 4
+        for (int64_t r = r0 + (threadIdx.x >> 5); r < r1; r += 8) {
+            const uint16_t *p = dgu + r * cols + c;
+            float v[PL][8];
+#pragma unroll
+            for (int t = 0; t < PL; ++t) load_vec<DT == STACR_DTYPE_F32 ? STACR_DTYPE_BF16 : DT, 8>(p + t * plane, v[t]);
+#pragma unroll
+            for (int e = 0; e < 8; ++e) {
+                if constexpr (PL == 3) sum[e] += v[0][e] + (v[1][e] + v[2][e]);
+                else sum[e] += v[0][e];
+            }
+        }
     }
-    part[(int64_t)blockIdx.y * cols + c] = sum;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) s[threadIdx.x >> 5][(threadIdx.x & 31) * 8 + e] = sum[e];
+    __syncthreads();
+    float v = 0.0f;
+#pragma unroll
+    for (int k = 0; k < 8; ++k) v += s[k][threadIdx.x];
+    const int64_t out = (int64_t)blockIdx.x * 256 + threadIdx.x;
+    if (out < cols) part[(int64_t)blockIdx.y * cols + out] = v;
 }
 
 template <int DT>
@@ -688,6 +778,7 @@ struct FewArgs {
     int64_t rows, d, x_ld, ff;
     int act;
     void *h, *gate, *up;
+    uint8_t *gate_low, *up_low;
 };
 
 // NT: blocks of 16 rows.  VEC: d and every row start are multiples of 8 values.
@@ -709,28 +800,40 @@ __global__ __launch_bounds__(kBlock) void k_gated_few(const FewArgs p)
     mmf4 ag[NT], au[NT];
 #pragma unroll
     for (int t = 0; t < NT; ++t) ag[t] = au[t] = mmf4{0.0f, 0.0f, 0.0f, 0.0f};
+    // U blocks of 32 of K a wave at a time, their loads all on the way before the first product (a loop over
+    // single blocks is not unrolled: matrix instructions do not allow a remainder loop).  One token through
+    // 1024 -> 4096: 7.7 us with one block at a time, 5.4 with eight.
+    constexpr int U = DT == STACR_DTYPE_F32 || !VEC ? 2 : NT == 4 ? 4 : 8;
     const int64_t d = p.d;
-#pragma unroll 4
-    for (int64_t k0 = wave * 32; k0 < d; k0 += kWaves * 32) {
-        const int64_t k = k0 + (lane >> 4) * 8, left = d - k;
-        uint4 g[P], u[P];
-        few_load<DT, VEC>(p.wg, f * d + k, left, g);
-        few_load<DT, VEC>(p.wu, f * d + k, left, u);
+    const auto blocks = [&](int64_t k0, auto whole) __attribute__((always_inline)) {
+        uint4 g[U][P], u[U][P], x[U][NT][P];
 #pragma unroll
-        for (int t = 0; t < NT; ++t) {
-            uint4 x[P];
-            few_load<DT, VEC>(p.x, xrow[t] + k, left, x);
-            if constexpr (DT == STACR_DTYPE_F32) {
+        for (int b = 0; b < U; ++b) {
+            const int64_t k = k0 + b * 32 + (lane >> 4) * 8, left = decltype(whole)::value ? 8 : d - k;
+            few_load<DT, VEC>(p.wg, f * d + k, left, g[b]);
+            few_load<DT, VEC>(p.wu, f * d + k, left, u[b]);
 #pragma unroll
-                for (int q = 0; q < kPairs; ++q) {
-                    ag[t] = mm_mfma<MT>(g[kPairB[q]], x[kPairA[q]], ag[t]);
-                    au[t] = mm_mfma<MT>(u[kPairB[q]], x[kPairA[q]], au[t]);
-                }
-            } else {
-                ag[t] = mm_mfma<MT>(g[0], x[0], ag[t]);
-                au[t] = mm_mfma<MT>(u[0], x[0], au[t]);
-            }
+            for (int t = 0; t < NT; ++t) few_load<DT, VEC>(p.x, xrow[t] + k, left, x[b][t]);
         }
+#pragma unroll
+        for (int b = 0; b < U; ++b)
+#pragma unroll
+            for (int t = 0; t < NT; ++t) {
+                if constexpr (DT == STACR_DTYPE_F32) {
+#pragma unroll
+                    for (int q = 0; q < kPairs; ++q) {
+                        ag[t] = mm_mfma<MT>(g[b][kPairB[q]], x[b][t][kPairA[q]], ag[t]);
+                        au[t] = mm_mfma<MT>(u[b][kPairB[q]], x[b][t][kPairA[q]], au[t]);
+                    }
+                } else {
+                    ag[t] = mm_mfma<MT>(g[b][0], x[b][t][0], ag[t]);
+                    au[t] = mm_mfma<MT>(u[b][0], x[b][t][0], au[t]);
+                }
+            }
+    };
+    for (int64_t k0 = wave * (U * 32); k0 < d; k0 += kWaves * (U * 32)) {
+        if (k0 + U * 32 <= d) blocks(k0, std::true_type());
+        else blocks(k0, std::false_type());
     }
 #pragma unroll
     for (int t = 0; t < NT; ++t)
@@ -752,8 +855,17 @@ __global__ __launch_bounds__(kBlock) void k_gated_few(const FewArgs p)
         activate<DT == STACR_DTYPE_F32>(p.act, g, a, slope);
         store_any(p.h, DT, m * p.ff + ff, a * u);
         if (p.gate) {
-            store_any(p.gate, DT, m * p.ff + ff, g);
-            store_any(p.up, DT, m * p.ff + ff, u);
+            const int64_t at = m * p.ff + ff;
+            if (DT != STACR_DTYPE_F32 && p.gate_low) {
+                const uint32_t x = to_24(g), y = to_24(u);
+                static_cast<uint16_t *>(p.gate)[at] = (uint16_t)(x >> 16);
+                static_cast<uint16_t *>(p.up)[at] = (uint16_t)(y >> 16);
+                p.gate_low[at] = (uint8_t)(x >> 8);
+                p.up_low[at] = (uint8_t)(y >> 8);
+            } else {
+                store_any(p.gate, DT, at, g);
+                store_any(p.up, DT, at, u);
+            }
         }
     }
 }
@@ -762,14 +874,13 @@ __global__ __launch_bounds__(kBlock) void k_gated_few(const FewArgs p)
 constexpr int64_t kFewRows = 64;
 
 // ------------------------------------------------------------------ host side
+constexpr int kCus = 256;
 constexpr int64_t kMaxFeatures = 1 << 20;  // row strides whose tile offsets stay within 31 bits
 
 inline int64_t up_to(int64_t n, int64_t m) { return (n + m - 1) / m * m; }
 inline size_t aligned(size_t n) { return (n + 255) & ~(size_t)255; }
 
 bool aligned_to(const void *p, size_t n) { return (reinterpret_cast<uintptr_t>(p) & (n - 1)) == 0; }
-
-int size_of(int dt) { return dt == STACR_DTYPE_F32 ? 4 : 2; }
 
 struct Problem {
     int dt;
@@ -787,27 +898,25 @@ Problem problem(int dt, int64_t rows, int64_t d, int64_t ff, int64_t x_ld, const
     return q;
 }
 
-template <typename K> void raise_lds(K kernel, size_t bytes)
+template <auto Kernel> void raise_lds(size_t bytes)
 {
-    static bool done = false;  // once per kernel instantiation
-    if (!done) {
-        (void)hipFuncSetAttribute(reinterpret_cast<const void *>(kernel), hipFuncAttributeMaxDynamicSharedMemorySize,
-                                  (int)bytes);
-        done = true;
-    }
+    static const hipError_t done = hipFuncSetAttribute(reinterpret_cast<const void *>(Kernel),
+                                                       hipFuncAttributeMaxDynamicSharedMemorySize, (int)bytes);
+    (void)done;  // a launch that it does not allow fails by itself
 }
 
 template <int DT, bool AK, bool BK, int EPI, int BM, int BN, int WM, int WN>
-void mm_run(MmArgs p, hipStream_t s)
+void mm_run(MmArgs p, int a_cu, hipStream_t s)
 {
-    constexpr size_t lds = mm_lds<DT, EPI, BM, BN>();
+    constexpr size_t lds = 2 * (BM + BN) * 128;
     static_assert(lds <= 160 * 1024, "LDS budget");
     p.mt = (int)((p.M + BM - 1) / BM);
     const int64_t cols = EPI == kBwd ? p.ff_pad : p.N;
     p.nt = (int)((cols + (EPI == kStore ? BN : BN / 2) - 1) / (EPI == kStore ? BN : BN / 2));
-    auto kernel = k_gated_mm<DT, AK, BK, EPI, BM, BN, WM, WN>;
-    raise_lds(kernel, lds);
-    const int grid = p.mt * p.nt * p.halves * p.splits;
+    p.tiles = p.mt * p.nt * p.halves * p.splits;
+    constexpr auto kernel = k_gated_mm<DT, AK, BK, EPI, BM, BN, WM, WN>;
+    raise_lds<kernel>(lds);
+    const int grid = hmin(p.tiles, kCus * a_cu);
     const char *name = EPI == kFwd ? "k_gated_mm_forward" : EPI == kBwd ? "k_gated_mm_slopes"
                        : BK || AK ? "k_gated_mm_input" : "k_gated_mm_weights";
     stacr_launch(name, s, [&] { kernel<<<grid, WM * WN * 64, lds, s>>>(p); });
@@ -815,42 +924,47 @@ void mm_run(MmArgs p, hipStream_t s)
 
 int64_t tiles(int64_t m, int64_t n, int bm, int bn) { return ((m + bm - 1) / bm) * ((n + bn - 1) / bn); }
 
-// Workgroups that share K of one tile: enough to give every CU one, as long as each keeps 16 steps (its
-// start and its partial product cost about that much).
-int splits_for(int64_t ntiles, int64_t steps)
-{
-    const int64_t want = 256 / (ntiles > 0 ? ntiles : 1), most = steps / 16;
-    const int64_t n = want < most ? want : most;
-    return n < 1 ? 1 : (int)n;
-}
-
-template <int DT, int EPI>
-void dual(const MmArgs &p, hipStream_t s)
-{
-    // 256 x 256 where its tiles fill the chip, else 128 x 128
-    if (tiles(p.M, p.N, 256, 128) >= 256) mm_run<DT, true, true, EPI, 256, 256, 2, 4>(p, s);
-    else mm_run<DT, true, true, EPI, 128, 128, 2, 2>(p, s);
-}
-
-template <int DT, bool AK>
-void product(MmArgs p, hipStream_t s, bool big)
-{
-    if (big) mm_run<DT, AK, false, kStore, 256, 256, 2, 4>(p, s);
-    else mm_run<DT, AK, false, kStore, 128, 128, 2, 2>(p, s);
-}
-
+// The tile of a product and how many workgroups share its K, by what they cost, in steps of a 256 x 256
+// tile (1.7 us): a round is as many tiles as the chip holds at once, a tile costs its steps and about 3 more
+// for its start and its results; partial products are written and read again (8192 x 1024 in two: 20 us).
+//   256 x 256   8 waves, one workgroup a CU: 1 a step
+//   256 x 128   8 waves, one workgroup a CU: 0.66 for half the work (LDS and L2 move 1.5 times as much for it)
+//   128 x 128   4 waves, two workgroups a CU: 0.62 for both, half the work together
+// (8192 x 1024 of K 8192, 128 tiles of 256 x 256: 130 us and 20 to join two splits; 256 of 256 x 128: 150 us;
+// 512 of 128 x 128: 130 to 142 us.)
 struct ProductPlan {
-    bool big;
-    int splits;
+    int tile, splits;
 };
 
-ProductPlan product_plan(int64_t m, int64_t n, int halves, int64_t k, int nseg)
+ProductPlan product_plan(int64_t m, int64_t n, int halves, int64_t k, int nseg, bool dual)
 {
-    const int64_t steps = (k + kMmK - 1) / kMmK * nseg;
-    ProductPlan q;
-    q.big = tiles(m, n, 256, 256) * halves >= 256;
-    q.splits = q.big ? 1 : splits_for(tiles(m, n, 128, 128) * halves, steps);
-    return q;
+    const int64_t steps = hmax<int64_t>(1, (k + kMmK - 1) / kMmK * nseg);
+    const double cost[3] = {1.0, 0.66, 0.62};
+    const int bm[3] = {256, 256, 128}, bn[3] = {256, 128, 128}, slots[3] = {kCus, kCus, 2 * kCus};
+    ProductPlan best{0, 1};
+    double least = 1e300;
+    for (int t = 0; t < 3; ++t) {
+        const int64_t each = tiles(m, n, bm[t], dual ? bn[t] / 2 : bn[t]) * halves;
+        for (int s = 1; s <= (dual ? 1 : 16) && s * 4 <= steps + 3; ++s) {
+            const int64_t rounds = (each * s + slots[t] - 1) / slots[t];
+            double c = rounds * ((double)((steps + s - 1) / s) + 3.0) * cost[t];
+            if (s > 1) c += 2.5 + (double)m * n * halves * 8.0 * s / 7.0e6 / 1.7;
+            if (c < least) least = c, best = ProductPlan{t, s};
+        }
+    }
+    return best;
+}
+
+template <int DT, bool AK, bool BK, int EPI> void tiled(const MmArgs &p, int tile, hipStream_t s)
+{
+    if (tile == 0) mm_run<DT, AK, BK, EPI, 256, 256, 2, 4>(p, 1, s);
+    else if (tile == 1) mm_run<DT, AK, BK, EPI, 256, 128, 4, 2>(p, 1, s);
+    else mm_run<DT, AK, BK, EPI, 128, 128, 2, 2>(p, 2, s);
+}
+
+template <int DT, int EPI> void dual(const MmArgs &p, hipStream_t s)
+{
+    tiled<DT, true, true, EPI>(p, product_plan(p.M, p.N, 1, p.K, p.nseg, true).tile, s);
 }
 
 size_t part_bytes(const ProductPlan &q, int64_t m, int64_t n, int halves)
@@ -882,8 +996,8 @@ Pieces pieces(const Problem &q, bool backward)
     if (backward) at += aligned((size_t)pl * q.rows * 2 * q.ff_pad * 2);
     w.part = at;
     if (backward) {
-        const size_t dx = part_bytes(product_plan(q.rows, q.d, 1, q.ff_pad, 2 * pairs(q.dt)), q.rows, q.d, 1);
-        const size_t dw = part_bytes(product_plan(q.ff, q.d, 2, q.rows, pairs(q.dt)), q.ff, q.d, 2);
+        const size_t dx = part_bytes(product_plan(q.rows, q.d, 1, q.ff_pad, 2 * pairs(q.dt), false), q.rows, q.d, 1);
+        const size_t dw = part_bytes(product_plan(q.ff, q.d, 2, q.rows, pairs(q.dt), false), q.ff, q.d, 2);
         const size_t db = aligned((size_t)((q.rows + kBiasRows - 1) / kBiasRows) * 2 * q.ff_pad * 4);
         at += hmax(hmax(dx, dw), db);
     }
@@ -996,10 +1110,8 @@ void product_typed(int dt, MmArgs p, const ProductPlan &plan, float *part, hipSt
     p.splits = plan.splits;
     p.part = part;
     p.out_dt = dt;
-    p.vec = p.N * size_of(dt) % 16 == 0 && aligned_to(p.out, 16) && aligned_to(p.out2, 16);
-    p.ldo = p.N;
-    if (dt == STACR_DTYPE_F16) product<STACR_DTYPE_F16, AK>(p, s, plan.big);
-    else product<STACR_DTYPE_BF16, AK>(p, s, plan.big);
+    if (dt == STACR_DTYPE_F16) tiled<STACR_DTYPE_F16, AK, false, kStore>(p, plan.tile, s);
+    else tiled<STACR_DTYPE_BF16, AK, false, kStore>(p, plan.tile, s);
     if (plan.splits > 1) {
         const int64_t half = p.M * p.N, n = half * p.halves;
         stacr_launch("k_gated_join", s, [&] {
@@ -1013,12 +1125,13 @@ void product_typed(int dt, MmArgs p, const ProductPlan &plan, float *part, hipSt
 }
 
 template <int DT>
-void slopes_launch(const void *dh, const void *gate, const void *up, const Problem &q, int act, uint16_t *dgu,
-                   int64_t plane, bool vec, hipStream_t s)
+void slopes_launch(const void *dh, const void *gate, const void *up, const uint8_t *gate_low, const uint8_t *up_low,
+                   const Problem &q, int act, uint16_t *dgu, int64_t plane, hipStream_t s)
 {
-    const int64_t n = q.rows * q.ff_pad / 4;
+    const int grid = blocks_for(q.rows * q.ff_pad / 8);
     stacr_launch("k_gated_slopes", s, [&] {
-        k_gated_slopes<DT><<<blocks_for(n), kBlock, 0, s>>>(dh, gate, up, q.rows, q.ff, act, dgu, q.ff_pad, plane, vec);
+        if (gate_low) k_gated_slopes<DT, true><<<grid, kBlock, 0, s>>>(dh, gate, up, gate_low, up_low, q.rows, q.ff, act, dgu, q.ff_pad, plane);
+        else k_gated_slopes<DT, false><<<grid, kBlock, 0, s>>>(dh, gate, up, nullptr, nullptr, q.rows, q.ff, act, dgu, q.ff_pad, plane);
     });
 }
 
@@ -1028,12 +1141,21 @@ void bias_launch(const uint16_t *dgu, const Problem &q, int64_t plane, float *pa
     const int parts = (int)((q.rows + kBiasRows - 1) / kBiasRows);
     if (parts)
         stacr_launch("k_gated_bias_part", s, [&] {
-            k_gated_bias_part<DT><<<dim3((unsigned)((2 * q.ff_pad + kBlock - 1) / kBlock), (unsigned)parts), kBlock, 0, s>>>(
+            k_gated_bias_part<DT><<<dim3((unsigned)((2 * q.ff_pad + 255) / 256), (unsigned)parts), kBlock, 0, s>>>(
                 dgu, q.rows, q.ff_pad, plane, part);
         });
     stacr_launch("k_gated_bias_sum", s, [&] {
         k_gated_bias_sum<DT><<<blocks_for(q.ff), kBlock, 0, s>>>(part, parts, q.ff, q.ff_pad, dbg, dbu);
     });
+}
+
+int check_kept(const char *what, int dtype, const void *gate, const void *up, const void *gate_low, const void *up_low)
+{
+    if ((gate == nullptr) != (up == nullptr) || (gate_low == nullptr) != (up_low == nullptr) || (gate_low && !gate))
+        return stacr_fail(STACR_ERR_INVALID, "%s: gate goes with up, gate_low with up_low, both with gate and up", what);
+    if (gate_low && dtype == STACR_DTYPE_F32)
+        return stacr_fail(STACR_ERR_INVALID, "%s: fp32 pre-activations have no low bytes", what);
+    return STACR_OK;
 }
 
 int check_problem(const char *what, int dtype, int64_t rows, int64_t d, int64_t ff, int64_t x_ld, int act)
@@ -1069,17 +1191,19 @@ int stacr_gated_workspace_bytes(const void *x, int dtype, int64_t rows, int64_t 
 
 int stacr_gated_forward(const void *x, int dtype, int64_t rows, int64_t d, int64_t x_ld, const void *w_gate,
                         const void *w_up, int64_t ff, const void *b_gate, const void *b_up, int activation, void *h,
-                        void *gate, void *up, void *workspace, size_t workspace_bytes, void *stream)
+                        void *gate, void *up, void *gate_low, void *up_low, void *workspace, size_t workspace_bytes, void *stream)
 {
     const int rc = check_problem("stacr_gated_forward", dtype, rows, d, ff, x_ld, activation);
     if (rc) return rc;
     if (rows == 0) return STACR_OK;
-    if (!x || !w_gate || !w_up || !h || (gate == nullptr) != (up == nullptr))
-        return stacr_fail(STACR_ERR_INVALID, "stacr_gated_forward: NULL pointer argument");
+    if (!x || !w_gate || !w_up || !h) return stacr_fail(STACR_ERR_INVALID, "stacr_gated_forward: NULL pointer argument");
+    const int kept = check_kept("stacr_gated_forward", dtype, gate, up, gate_low, up_low);
+    if (kept) return kept;
     hipStream_t s = static_cast<hipStream_t>(stream);
     Problem q = problem(dtype, rows, d, ff, x_ld, x, w_gate, w_up);
     if (rows <= kFewRows) {
-        const FewArgs a{x, w_gate, w_up, b_gate, b_up, rows, d, x_ld, ff, activation, h, gate, up};
+        const FewArgs a{x, w_gate, w_up, b_gate, b_up, rows, d, x_ld, ff, activation, h, gate, up,
+                        static_cast<uint8_t *>(gate_low), static_cast<uint8_t *>(up_low)};
         const bool vec = d % 8 == 0 && x_ld % 8 == 0 && aligned_to(x, 16) && aligned_to(w_gate, 16) && aligned_to(w_up, 16);
         if (dtype == STACR_DTYPE_F32) few_typed<STACR_DTYPE_F32>(a, vec, s);
         else if (dtype == STACR_DTYPE_BF16) few_typed<STACR_DTYPE_BF16>(a, vec, s);
@@ -1095,21 +1219,24 @@ int stacr_gated_forward(const void *x, int dtype, int64_t rows, int64_t d, int64
     p.out = h;
     p.gate = gate;
     p.up = up;
-    p.vec = ff * size_of(dtype) % 16 == 0 && aligned_to(h, 16) && aligned_to(gate, 16) && aligned_to(up, 16);
+    p.gate_low = static_cast<uint8_t *>(gate_low);
+    p.up_low = static_cast<uint8_t *>(up_low);
     dual_typed<kFwd>(dtype, p, s);
     return stacr_hip_check(hipGetLastError(), "gated forward kernels");
 }
 
 int stacr_gated_backward(const void *dh, const void *x, int dtype, int64_t rows, int64_t d, int64_t x_ld,
                          const void *w_gate, const void *w_up, int64_t ff, const void *b_gate, const void *b_up,
-                         int activation, const void *gate, const void *up, void *dx, void *dw_gate, void *dw_up,
+                         int activation, const void *gate, const void *up, const void *gate_low, const void *up_low,
+                         void *dx, void *dw_gate, void *dw_up,
                          void *db_gate, void *db_up, void *dgu, void *workspace, size_t workspace_bytes, void *stream)
 {
     const int rc = check_problem("stacr_gated_backward", dtype, rows, d, ff, x_ld, activation);
     if (rc) return rc;
     const bool kept = gate != nullptr, weights = dw_gate != nullptr;
-    if ((gate == nullptr) != (up == nullptr) || weights != (dw_up != nullptr))
-        return stacr_fail(STACR_ERR_INVALID, "stacr_gated_backward: gate with up and dw_gate with dw_up");
+    if (weights != (dw_up != nullptr)) return stacr_fail(STACR_ERR_INVALID, "stacr_gated_backward: dw_gate with dw_up");
+    const int bad = check_kept("stacr_gated_backward", dtype, gate, up, gate_low, up_low);
+    if (bad) return bad;
     if (rows && (!dh || (!x && (!kept || weights)) || ((!w_gate || !w_up) && (!kept || dx))))
         return stacr_fail(STACR_ERR_INVALID, "stacr_gated_backward: NULL pointer argument");
     if (dgu && dtype == STACR_DTYPE_F32)
@@ -1127,17 +1254,16 @@ int stacr_gated_backward(const void *dh, const void *x, int dtype, int64_t rows,
     uint16_t *slopes = dgu ? static_cast<uint16_t *>(dgu) : reinterpret_cast<uint16_t *>(ws + w.dgu);
     float *part = reinterpret_cast<float *>(ws + w.part);
     const Operands o = operands(q, x, w_gate, w_up, ws, w, rows > 0 && (!kept || weights), rows > 0 && (!kept || dx), s);
-    const bool vec = ff * size_of(dtype) % 16 == 0 && aligned_to(dh, 16) && aligned_to(gate, 16) && aligned_to(up, 16);
     if (rows && kept) {
-        if (dtype == STACR_DTYPE_F32) slopes_launch<STACR_DTYPE_F32>(dh, gate, up, q, activation, slopes, plane, vec, s);
-        else if (dtype == STACR_DTYPE_BF16) slopes_launch<STACR_DTYPE_BF16>(dh, gate, up, q, activation, slopes, plane, vec, s);
-        else slopes_launch<STACR_DTYPE_F16>(dh, gate, up, q, activation, slopes, plane, vec, s);
+        const uint8_t *gl = static_cast<const uint8_t *>(gate_low), *ul = static_cast<const uint8_t *>(up_low);
+        if (dtype == STACR_DTYPE_F32) slopes_launch<STACR_DTYPE_F32>(dh, gate, up, nullptr, nullptr, q, activation, slopes, plane, s);
+        else if (dtype == STACR_DTYPE_BF16) slopes_launch<STACR_DTYPE_BF16>(dh, gate, up, gl, ul, q, activation, slopes, plane, s);
+        else slopes_launch<STACR_DTYPE_F16>(dh, gate, up, gl, ul, q, activation, slopes, plane, s);
     } else if (rows) {
         MmArgs p = gated_args(q, o, b_gate, b_up, activation);
         p.dh = dh;
         p.dgu = slopes;
         p.plane = plane;
-        p.vec = vec;
         dual_typed<kBwd>(dtype, p, s);
     }
     const int np = pairs(dtype);
@@ -1159,9 +1285,15 @@ int stacr_gated_backward(const void *dh, const void *x, int dtype, int64_t rows,
         p.K = ff;
         p.halves = 1;
         p.out = dx;
-        product_typed<true>(dtype, p, product_plan(rows, d, 1, q.ff_pad, p.nseg), part, s);
+        product_typed<true>(dtype, p, product_plan(rows, d, 1, q.ff_pad, p.nseg, false), part, s);
     }
-    if (weights) {
+    if (weights && rows == 0) {
+        const int bytes = dtype == STACR_DTYPE_F32 ? 4 : 2;
+        for (void *w : {dw_gate, dw_up}) {
+            const int e = stacr_fill_int_launch(w, bytes, ff * d, 0, s);
+            if (e) return e;
+        }
+    } else if (weights) {
         MmArgs p{};
         p.nseg = np;
         for (int i = 0; i < np; ++i) {
@@ -1179,7 +1311,7 @@ int stacr_gated_backward(const void *dh, const void *x, int dtype, int64_t rows,
         p.halves = 2;
         p.out = dw_gate;
         p.out2 = dw_up;
-        product_typed<false>(dtype, p, product_plan(ff, d, 2, rows, np), part, s);
+        product_typed<false>(dtype, p, product_plan(ff, d, 2, rows, np, false), part, s);
     }
     if (db_gate || db_up) {
         if (dtype == STACR_DTYPE_F32) bias_launch<STACR_DTYPE_F32>(slopes, q, plane, part, db_gate, db_up, s);

@@ -92,9 +92,10 @@ SIGNATURES = {
     "stacr_c1_observe": ([_p, _i32, _i64, _i64, _p, _p, _i32, _i32, _p, _p, _p, _sz, _p], _i32),
     "stacr_c1_store": ([_p, _i64, _i32, _p, _i32, _p, _i32, _p], _i32),
     "stacr_gated_workspace_bytes": ([_p, _i32, _i64, _i64, _i64, _p, _p, _i64, _i32, _PSZ], _i32),
-    "stacr_gated_forward": ([_p, _i32, _i64, _i64, _i64, _p, _p, _i64, _p, _p, _i32, _p, _p, _p, _p, _sz, _p], _i32),
+    "stacr_gated_forward": ([_p, _i32, _i64, _i64, _i64, _p, _p, _i64, _p, _p, _i32, _p, _p, _p, _p, _p, _p, _sz, _p],
+                            _i32),
     "stacr_gated_backward": ([_p, _p, _i32, _i64, _i64, _i64, _p, _p, _i64, _p, _p, _i32, _p, _p, _p, _p, _p, _p, _p,
-                              _p, _p, _sz, _p], _i32),
+                              _p, _p, _p, _p, _sz, _p], _i32),
     "stacr_rotary_tables": ([_i64, _i32, _f64, _i32, _f64, _i64, _f64, _f64, _p, _p, _p], _i32),
     "stacr_rotary": ([_p, _p, _i32, _p, _p, _i32, _i32, _i64, _i64, _i32, _i32, _i32, _p, _p, _i64, _p, _i32, _i64, _i64, _i64,
                       _i32, _p, _p, _p, _p, _p], _i32),

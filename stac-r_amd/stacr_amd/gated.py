@@ -1,7 +1,7 @@
 """The gated feed-forward block h = act(x Wg^T + bg) * (x Wu^T + bu) and its gradients in HIP kernels.
 
 ``gated_feed_forward`` is the exact operator: one kernel forms both projections, the activation and the
-product, and nothing but the input is kept for the backward, which forms the pre-activations again.
+product.
 (No counterpart in the reference, whose layers wrap the projections one by one.)
 """
 from __future__ import annotations
@@ -41,36 +41,51 @@ def _contiguous(t):
 
 
 class GatedFeedForwardFunction(torch.autograd.Function):
-    """Saved tensors: the input, both weights and the biases (all of them the caller's own)."""
+    """Saved tensors: the input, both weights, the biases (all of them the caller's own) and, unless the
+    backward is to compute them again, the pre-activations."""
 
     @staticmethod
-    def forward(ctx, x, w_gate, w_up, b_gate, b_up, activation):
-        ctx.save_for_backward(x, w_gate, w_up, b_gate, b_up)
+    def forward(ctx, x, w_gate, w_up, b_gate, b_up, activation, recompute):
+        x2d = x if x.dim() == 2 else x.reshape(-1, x.shape[-1])
+        h = kernels.gated_forward(x2d, w_gate, w_up, _contiguous(b_gate), _contiguous(b_up), activation,
+                                  None if recompute else "full")
+        kept = (None,) * 4
+        if not recompute:
+            h, kept = h
+        ctx.save_for_backward(x, w_gate, w_up, b_gate, b_up, *kept)
         ctx.activation = activation
-        h = kernels.gated_forward(x.reshape(-1, x.shape[-1]), w_gate, w_up, _contiguous(b_gate), _contiguous(b_up),
-                                  activation)
-        return h.view(*x.shape[:-1], h.shape[1])
+        return h if x.dim() == 2 else h.view(*x.shape[:-1], h.shape[1])
 
     @staticmethod
     @once_differentiable
     def backward(ctx, dh):
-        x, w_gate, w_up, b_gate, b_up = ctx.saved_tensors
+        x, w_gate, w_up, b_gate, b_up, *kept = ctx.saved_tensors
         need = ctx.needs_input_grad
+        if x.dim() != 2:
+            dh, x2d = dh.reshape(-1, dh.shape[-1]), x.reshape(-1, x.shape[-1])
+        else:
+            x2d = x
         dx, dwg, dwu, dbg, dbu, _ = kernels.gated_backward(
-            dh.reshape(-1, dh.shape[-1]), x.reshape(-1, x.shape[-1]), w_gate, w_up, _contiguous(b_gate),
-            _contiguous(b_up), ctx.activation, needs=(need[0], need[1] or need[2], need[3], need[4]))
-        return (dx.view(x.shape) if dx is not None else None, dwg if need[1] else None, dwu if need[2] else None, dbg,
-                dbu, None)
+            dh, x2d, w_gate, w_up, _contiguous(b_gate), _contiguous(b_up), ctx.activation,
+            None if kept[0] is None else kept, (need[0], need[1] or need[2], need[3], need[4]))
+        if dx is not None and x.dim() != 2:
+            dx = dx.view(x.shape)
+        return dx, dwg if need[1] else None, dwu if need[2] else None, dbg, dbu, None, None
 
 
 def gated_feed_forward(x: torch.Tensor, w_gate: torch.Tensor, w_up: torch.Tensor, b_gate: torch.Tensor | None = None,
-                       b_up: torch.Tensor | None = None, *, activation: str = "silu") -> torch.Tensor:
+                       b_up: torch.Tensor | None = None, *, activation: str = "silu",
+                       recompute: bool = False) -> torch.Tensor:
     """act(x w_gate^T + b_gate) * (x w_up^T + b_up) over the last dimension of ``x``, differentiable.
 
     Weights as nn.Linear keeps them, (ff, d); one of float32, bfloat16, float16 throughout (under
     autocast everything is cast to its type first).  ``activation``: "silu", "gelu", "gelu_tanh", "relu"
     or "sigmoid".  Sums in fp32, one rounding at the end; the backward rounds dg and du to the type
     between its products.
+
+    For the backward the two pre-activations are kept, in 24 bits each (fp32: 32), which costs what eager
+    16-bit training keeps of this block (g, act(g) and u).  ``recompute=True`` keeps nothing but the input
+    and forms them again in the backward: the same gradients up to the 24 bits' rounding, at a third more work.
     """
     if torch.is_autocast_enabled(x.device.type):
         dtype = torch.get_autocast_dtype(x.device.type)
@@ -79,7 +94,7 @@ def gated_feed_forward(x: torch.Tensor, w_gate: torch.Tensor, w_up: torch.Tensor
     if torch.is_grad_enabled() and (x.requires_grad or w_gate.requires_grad or w_up.requires_grad or
                                     (b_gate is not None and b_gate.requires_grad) or
                                     (b_up is not None and b_up.requires_grad)):
-        return GatedFeedForwardFunction.apply(x, w_gate, w_up, b_gate, b_up, activation)
+        return GatedFeedForwardFunction.apply(x, w_gate, w_up, b_gate, b_up, activation, recompute)
     if x.dim() == 2:
         return kernels.gated_forward(x, w_gate, w_up, _contiguous(b_gate), _contiguous(b_up), activation)
     h = kernels.gated_forward(x.reshape(-1, x.shape[-1]), w_gate, w_up, _contiguous(b_gate), _contiguous(b_up),

@@ -605,31 +605,36 @@ def _rows_of(x2d):
 
 
 def gated_forward(x2d: torch.Tensor, w_gate: torch.Tensor, w_up: torch.Tensor, b_gate: torch.Tensor | None = None,
-                  b_up: torch.Tensor | None = None, activation: str = "silu", keep: bool = False):
-    """h = act(x Wg^T + bg) * (x Wu^T + bu) of rows x d (stacr_gated_forward); with ``keep`` (h, g, u), the
-    pre-activations rounded to the type.  The caller has checked shapes, types and devices
-    (gated.gated_feed_forward does)."""
+                  b_up: torch.Tensor | None = None, activation: str = "silu", keep: str | None = None):
+    """h = act(x Wg^T + bg) * (x Wu^T + bu) of rows x d (stacr_gated_forward).  ``keep`` "type" or "full": also
+    the pre-activations for gated_backward, (h, kept): rounded to the type, or 16-bit types in 24 bits.  The
+    caller has checked shapes, types and devices (gated.gated_feed_forward does)."""
     x2d, x_ld = _rows_of(x2d)
     w_gate, w_up = w_gate.contiguous(), w_up.contiguous()
     rows, d = x2d.shape
     ff = w_gate.shape[0]
     code = dtype_code(x2d.dtype)
     h = x2d.new_empty((rows, ff))
-    gate, up = (torch.empty_like(h), torch.empty_like(h)) if keep else (None, None)
+    gate = up = gate_low = up_low = None
+    if keep is not None:
+        gate, up = torch.empty_like(h), torch.empty_like(h)
+        if keep == "full" and code != _lib.DTYPE_F32:
+            gate_low, up_low = (torch.empty((rows, ff), dtype=torch.uint8, device=h.device) for _ in range(2))
     ws, nbytes = (None, 0) if rows <= GATED_FEW_ROWS else _gated_workspace(x2d, code, rows, d, x_ld, w_gate, w_up, 0)
     rc = _lib.load().stacr_gated_forward(x2d.data_ptr(), code, rows, d, x_ld, w_gate.data_ptr(), w_up.data_ptr(), ff,
                                          _at(b_gate), _at(b_up), _lib.ACTIVATION_CODES[activation], h.data_ptr(),
-                                         _at(gate), _at(up), _at(ws), nbytes, _raw_stream(x2d))
+                                         _at(gate), _at(up), _at(gate_low), _at(up_low), _at(ws), nbytes,
+                                         _raw_stream(x2d))
     if rc:
         _lib.check(rc, "stacr_gated_forward")
-    return (h, gate, up) if keep else h
+    return h if keep is None else (h, (gate, up, gate_low, up_low))
 
 
 def gated_backward(dh: torch.Tensor, x2d: torch.Tensor | None, w_gate: torch.Tensor, w_up: torch.Tensor,
                    b_gate: torch.Tensor | None = None, b_up: torch.Tensor | None = None, activation: str = "silu",
                    kept=None, needs=(True, True, False, False), slopes: bool = False):
     """(dx, dw_gate, dw_up, db_gate, db_up, dgu) for dh, None where ``needs`` (input, weights, gate bias, up
-    bias) asks for none (stacr_gated_backward).  ``kept``: (g, u) of the forward, or None to compute them
+    bias) asks for none (stacr_gated_backward).  ``kept``: what gated_forward kept, or None to compute it
     again from x2d, which may be None with them when no weight gradient is asked for.  ``slopes``: give
     out dgu = [dg | du], rows x 2 p with p = ff rounded up to 8 (16-bit types)."""
     dh, w_gate, w_up = dh.contiguous(), w_gate.contiguous(), w_up.contiguous()
@@ -642,12 +647,13 @@ def gated_backward(dh: torch.Tensor, x2d: torch.Tensor | None, w_gate: torch.Ten
     dbg = dh.new_empty(ff) if needs[2] else None
     dbu = dh.new_empty(ff) if needs[3] else None
     dgu = dh.new_empty((rows, 2 * ((ff + 7) // 8 * 8))) if slopes else None
-    gate, up = kept if kept is not None else (None, None)
+    gate, up, gate_low, up_low = kept if kept is not None else (None,) * 4
     ws, nbytes = _gated_workspace(x2d, code, rows, d, x_ld, w_gate, w_up, 1)
     rc = _lib.load().stacr_gated_backward(dh.data_ptr(), _at(x2d), code, rows, d, x_ld, w_gate.data_ptr(),
                                           w_up.data_ptr(), ff, _at(b_gate), _at(b_up),
-                                          _lib.ACTIVATION_CODES[activation], _at(gate), _at(up), _at(dx), _at(dwg),
-                                          _at(dwu), _at(dbg), _at(dbu), _at(dgu), _at(ws), nbytes, _raw_stream(dh))
+                                          _lib.ACTIVATION_CODES[activation], _at(gate), _at(up), _at(gate_low),
+                                          _at(up_low), _at(dx), _at(dwg), _at(dwu), _at(dbg), _at(dbu), _at(dgu),
+                                          _at(ws), nbytes, _raw_stream(dh))
     if rc:
         _lib.check(rc, "stacr_gated_backward")
     return dx, dwg, dwu, dbg, dbu, dgu

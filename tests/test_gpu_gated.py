@@ -82,11 +82,16 @@ def tolerance(dtype, sums, gradient):
 
 
 def check(tensors, dh, act, dtype):
+    for recompute in (False, True):
+        check_form(tensors, dh, act, dtype, recompute)
+
+
+def check_form(tensors, dh, act, dtype, recompute):
     import stacr_amd
 
     h64, g64 = formula(tensors, dh, act)
     leaves = [None if t is None else t.detach().requires_grad_(True) for t in tensors]
-    h = stacr_amd.gated_feed_forward(*leaves, activation=act)
+    h = stacr_amd.gated_feed_forward(*leaves, activation=act, recompute=recompute)
     rows, d, ff = h.shape[0], tensors[1].shape[1], tensors[1].shape[0]
     assert off(h.detach(), h64) <= tolerance(dtype, d, False)
     with torch.no_grad():  # the form without a backward is the same kernel
@@ -274,12 +279,13 @@ def test_kept_preactivations(dev, rows, d, ff, dtype):
 
     announce("gated kept", rows, d, ff, dtype)
     (x, wg, wu, bg, bu), dh = make(rows, d, ff, dtype, dev)
-    h, g, u = kernels.gated_forward(x, wg, wu, bg, bu, "silu", keep=True)
+    h, kept = kernels.gated_forward(x, wg, wu, bg, bu, "silu", keep="type")
+    g = kept[0]
     assert torch.equal(h, kernels.gated_forward(x, wg, wu, bg, bu, "silu"))
     g64 = x.double() @ wg.double().t() + bg.double()
     assert off(g, g64) <= tolerance(dtype, d, False)
     give = dtype != "f32"
-    dx, dwg, dwu, dbg, dbu, dgu = kernels.gated_backward(dh, x, wg, wu, bg, bu, "silu", kept=(g, u),
+    dx, dwg, dwu, dbg, dbu, dgu = kernels.gated_backward(dh, x, wg, wu, bg, bu, "silu", kept=kept,
                                                          needs=(True, True, True, True), slopes=give)
     _, want = formula([x, wg, wu, bg, bu], dh, "silu")
     room = 1.5 if give else 1.0
@@ -288,7 +294,7 @@ def test_kept_preactivations(dev, rows, d, ff, dtype):
     if give:
         pad = (ff + 7) // 8 * 8
         assert dgu.shape == (rows, 2 * pad) and not dgu[:, ff:pad].any() and not dgu[:, pad + ff:].any()
-        alone = kernels.gated_backward(dh, None, wg, wu, bg, bu, "silu", kept=(g, u), needs=(True, False, False, False),
+        alone = kernels.gated_backward(dh, None, wg, wu, bg, bu, "silu", kept=kept, needs=(True, False, False, False),
                                        slopes=True)
         assert torch.equal(alone[0], dx) and torch.equal(alone[5], dgu)
 
