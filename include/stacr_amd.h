@@ -504,10 +504,10 @@ int stacr_qr_tall(const float *a, int64_t rows, int cols, float *q, float *r, vo
  * Gated feed-forward block (no counterpart in the reference, whose layers wrap its projections):
  *   g = x Wg^T + bg, u = x Wu^T + bu, h = act(g) * u
  * x: rows x d with rows x_ld >= d values apart; w_gate, w_up: ff x d (row-major, as nn.Linear keeps
- * them); biases ff values or NULL; h: rows x ff.  gate and up (both or NULL; rows x ff) keep g and u for
- * the backward: rounded to the type, or with gate_low and up_low (bytes, rows x ff; 16-bit types) in 24
- * bits, the upper 16 bits of the fp32 value in gate / up and the next 8 in the low bytes.  One
- * type throughout; sums in fp32 (fp32 inputs: to fp32 accuracy).  The workspace holds operands whose
+ * them); biases ff values or NULL; h: rows x ff.  gate and up (both or NULL; rows of p values, p = ff
+ * rounded up to 8, 16-byte aligned) keep g and u for the backward: rounded to the type, or with gate_low and
+ * up_low (the same shape, bytes; 16-bit types) in 24 bits, the upper 16 bits of the fp32 value in gate /
+ * up and the next 8 in the low bytes.  One type throughout; sums in fp32 (fp32 inputs: to fp32 accuracy).  The workspace holds operands whose
  * rows are not whole, aligned groups of 8 values in another form (fp32: always), so its size depends on
  * the pointers' alignment, which is all that the query looks at.  rows 0 is a no-op.  d, ff and x_ld at
  * most 2^20, rows below 2^24 (STACR_ERR_UNSUPPORTED).

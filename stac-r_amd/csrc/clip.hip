@@ -6,8 +6,8 @@
 // by 1 would change nothing.  Sums in 64 bits: squares of fp32 neither overflow nor vanish there, and a
 // sum over 10^9 values keeps all its digits.
 //
-// Tensors come as pointers and lengths in the kernel's own arguments (4 KiB: about 120 tensors a
-// launch), so nothing is copied to the device and a call can be captured into a graph.  The tensors
+// Tensors come as pointers and lengths in the kernel's own arguments (4 KiB: 272 tensors a launch, 176
+// with outputs of their own), so nothing is copied to the device and a call can be captured into a graph.  The tensors
 // are cut into chunks of 8192 elements and a workgroup takes a range of chunks, so of each tensor one
 // run of elements; a chunk's loads are under way while the one before it is worked on.
 #include "internal.h"
@@ -16,25 +16,29 @@ using namespace stacr;
 
 namespace {
 
-constexpr int kTensors = 120;           // of a launch
 constexpr int kChunk = 8192;            // elements: 256 threads x 4 pieces of 8
 constexpr int kPieces = kChunk / (kBlock * 8);
-constexpr int kGroups = 1024;           // workgroups of a pass over all its launches, 4 a CU
+// Workgroups of a launch, 4 a CU.  (Shared out over a call's launches, a third of them each, the norm of
+// 266 tensors ran at 3.6 TB/s; one launch with all of them reads at 5.6.)
+constexpr int kGroups = 1024;
 
-struct ClipArgs {
-    const void *in[kTensors];
-    void *out[kTensors];
-    int64_t n[kTensors];
-    uint32_t first[kTensors];           // first chunk of the tensor in this launch
-    uint32_t dtype[kTensors];
+// The tensors of a launch, at most T, and with outputs of their own where OUT (otherwise in place).
+template <int T, bool OUT> struct Table {
+    static constexpr int kTensors = T;
+    static constexpr bool kOut = OUT;
+    const void *in[T];
+    void *out[OUT ? T : 1];
+    uint32_t first[T + 1];              // first chunk of each, and the end
+    uint16_t tail[T];                   // elements of the last chunk (1 .. 8192) | type << 14
     int count;
-    uint32_t chunks;
     int parts;                          // partial norms over all launches
     double *part;                       // the norm pass: this launch's
     double max_norm, eps;
     float *norm_out;                    // or NULL
 };
-static_assert(sizeof(ClipArgs) <= 4096, "kernel arguments");
+using Alone = Table<272, false>;
+using Pairs = Table<176, true>;
+static_assert(sizeof(Alone) <= 4096 && sizeof(Pairs) <= 4096, "kernel arguments");
 
 struct Raw8 {  // eight elements as they lie in memory
     uint4 w[2];
@@ -137,11 +141,12 @@ __device__ __forceinline__ void run_scale(const void *in, void *out, int64_t fro
     }
 }
 
-// f(tensor, first element, end) over this workgroup's runs
-template <typename F> __device__ __forceinline__ void over_runs(const ClipArgs &a, F &&f)
+// f(tensor, its type, first element, end) over this workgroup's runs
+template <typename A, typename F> __device__ __forceinline__ void over_runs(const A &a, F &&f)
 {
-    uint32_t c = (uint32_t)((uint64_t)a.chunks * blockIdx.x / gridDim.x);
-    const uint32_t end = (uint32_t)((uint64_t)a.chunks * (blockIdx.x + 1) / gridDim.x);
+    const uint32_t chunks = a.first[a.count];
+    uint32_t c = (uint32_t)((uint64_t)chunks * blockIdx.x / gridDim.x);
+    const uint32_t end = (uint32_t)((uint64_t)chunks * (blockIdx.x + 1) / gridDim.x);
     if (c >= end) return;
     int t = 0, hi = a.count - 1;  // the last tensor that starts at or before chunk c
     while (t < hi) {
@@ -150,9 +155,10 @@ template <typename F> __device__ __forceinline__ void over_runs(const ClipArgs &
         else hi = mid - 1;
     }
     for (; c < end; ++t) {
-        const uint32_t first = a.first[t], stop = t + 1 < a.count && a.first[t + 1] < end ? a.first[t + 1] : end;
-        const int64_t to = (int64_t)(stop - first) * kChunk;
-        f(t, (int64_t)(c - first) * kChunk, to < a.n[t] ? to : a.n[t]);
+        const uint32_t first = a.first[t], next = a.first[t + 1], stop = next < end ? next : end;
+        const uint32_t tail = a.tail[t];
+        const int64_t n = (int64_t)(next - first - 1) * kChunk + (tail & 0x3fffu), to = (int64_t)(stop - first) * kChunk;
+        f(t, tail >> 14, (int64_t)(c - first) * kChunk, to < n ? to : n);
         c = stop;
     }
 }
@@ -177,20 +183,20 @@ template <int NORM> __device__ __forceinline__ double block_join(double v)
     return v;
 }
 
-template <int NORM> __global__ __launch_bounds__(kBlock) void k_grad_norm(const ClipArgs a)
+template <int NORM> __global__ __launch_bounds__(kBlock) void k_grad_norm(const Alone a)
 {
     double sum = 0.0;
     uint32_t top = 0;
-    over_runs(a, [&](int t, int64_t from, int64_t to) {
-        if (a.dtype[t] == STACR_DTYPE_F32) run_norm<STACR_DTYPE_F32, NORM>(a.in[t], from, to, sum, top);
-        else if (a.dtype[t] == STACR_DTYPE_BF16) run_norm<STACR_DTYPE_BF16, NORM>(a.in[t], from, to, sum, top);
+    over_runs(a, [&](int t, uint32_t type, int64_t from, int64_t to) {
+        if (type == STACR_DTYPE_F32) run_norm<STACR_DTYPE_F32, NORM>(a.in[t], from, to, sum, top);
+        else if (type == STACR_DTYPE_BF16) run_norm<STACR_DTYPE_BF16, NORM>(a.in[t], from, to, sum, top);
         else run_norm<STACR_DTYPE_F16, NORM>(a.in[t], from, to, sum, top);
     });
     const double v = block_join<NORM>(NORM == 0 ? (double)__uint_as_float(top) : sum);
     if (threadIdx.x == 0) a.part[blockIdx.x] = v;
 }
 
-template <int NORM> __global__ __launch_bounds__(kBlock) void k_grad_clip(const ClipArgs a)
+template <int NORM, typename A> __global__ __launch_bounds__(kBlock) void k_grad_clip(const A a)
 {
     double v = 0.0;
 #pragma unroll 8
@@ -203,17 +209,60 @@ template <int NORM> __global__ __launch_bounds__(kBlock) void k_grad_clip(const 
     double f = a.max_norm / (norm + a.eps);
     if (f > 1.0) f = 1.0;
     const float factor = (float)f;
-    over_runs(a, [&](int t, int64_t from, int64_t to) {
-        if (factor == 1.0f && a.in[t] == a.out[t]) return;
-        if (a.dtype[t] == STACR_DTYPE_F32) run_scale<STACR_DTYPE_F32>(a.in[t], a.out[t], from, to, factor);
-        else if (a.dtype[t] == STACR_DTYPE_BF16) run_scale<STACR_DTYPE_BF16>(a.in[t], a.out[t], from, to, factor);
-        else run_scale<STACR_DTYPE_F16>(a.in[t], a.out[t], from, to, factor);
+    if (!A::kOut && factor == 1.0f) return;
+    over_runs(a, [&](int t, uint32_t type, int64_t from, int64_t to) {
+        void *out = A::kOut ? a.out[A::kOut ? t : 0] : const_cast<void *>(a.in[t]);
+        if (factor == 1.0f && a.in[t] == out) return;
+        if (type == STACR_DTYPE_F32) run_scale<STACR_DTYPE_F32>(a.in[t], out, from, to, factor);
+        else if (type == STACR_DTYPE_BF16) run_scale<STACR_DTYPE_BF16>(a.in[t], out, from, to, factor);
+        else run_scale<STACR_DTYPE_F16>(a.in[t], out, from, to, factor);
     });
 }
 
 int64_t chunks_of(int64_t n) { return (n + kChunk - 1) / kChunk; }
 
-int launches_for(int count) { return (count + kTensors - 1) / kTensors; }
+// the launch of tensors from `i` on, as many as fit of those that hold anything; i moves past them
+template <typename A>
+void fill(A &a, int &i, int count, const void *const *in, void *const *out, const int64_t *sizes, const int *dtypes)
+{
+    a.count = 0;
+    a.first[0] = 0;
+    for (; i < count && a.count < A::kTensors; ++i) {
+        if (!sizes[i]) continue;
+        const int64_t chunks = chunks_of(sizes[i]);
+        a.in[a.count] = in[i];
+        if (A::kOut) a.out[a.count] = out[i];
+        a.tail[a.count] = (uint16_t)((sizes[i] - (chunks - 1) * kChunk) | dtypes[i] << 14);
+        a.first[a.count + 1] = a.first[a.count] + (uint32_t)chunks;
+        ++a.count;
+    }
+}
+
+template <typename A> int groups(const A &a) { return (int)hmin<int64_t>(kGroups, a.first[a.count]); }
+
+template <typename A>
+void clip_launches(int norm_type, int count, const void *const *in, void *const *out, const int64_t *sizes, const int *dtypes,
+                   double max_norm, double eps, double *part, int parts, float *norm, hipStream_t s)
+{
+    A a{};
+    a.max_norm = max_norm;
+    a.eps = eps;
+    a.part = part;
+    a.parts = parts;
+    a.norm_out = norm;
+    int i = 0;
+    do {
+        if (out) fill(a, i, count, in, out, sizes, dtypes);
+        const int grid = a.count ? groups(a) : 1;  // none: the norm alone
+        if (a.count || a.norm_out)
+            stacr_launch("k_grad_clip", s, [&] {
+                if (norm_type == 2) k_grad_clip<2, A><<<grid, kBlock, 0, s>>>(a);
+                else if (norm_type == 1) k_grad_clip<1, A><<<grid, kBlock, 0, s>>>(a);
+                else k_grad_clip<0, A><<<grid, kBlock, 0, s>>>(a);
+            });
+        a.norm_out = nullptr;
+    } while (out && i < count);
+}
 
 }  // namespace
 
@@ -222,7 +271,7 @@ extern "C" {
 int stacr_clip_workspace_bytes(int count, size_t *bytes)
 {
     if (count < 0 || !bytes) return stacr_fail(STACR_ERR_INVALID, "stacr_clip_workspace_bytes: bad argument");
-    *bytes = sizeof(double) * (size_t)(kGroups + launches_for(count) + 1);
+    *bytes = sizeof(double) * (size_t)kGroups * (size_t)((count + Alone::kTensors - 1) / Alone::kTensors + 1);
     return STACR_OK;
 }
 
@@ -253,31 +302,10 @@ int stacr_clip_gradients(int count, const void *const *in, void *const *out, con
     hipStream_t s = static_cast<hipStream_t>(stream);
     double *part = static_cast<double *>(workspace);
 
-    // the launch of tensors from `first` on: at most kTensors that hold anything; returns the next first
-    const auto fill = [&](ClipArgs &a, int first) {
-        a.count = 0;
-        a.chunks = 0;
-        int i = first;
-        for (; i < count && a.count < kTensors; ++i) {
-            if (!sizes[i]) continue;
-            a.in[a.count] = in[i];
-            a.out[a.count] = out ? out[i] : nullptr;
-            a.n[a.count] = sizes[i];
-            a.dtype[a.count] = (uint32_t)dtypes[i];
-            a.first[a.count++] = a.chunks;
-            a.chunks += (uint32_t)chunks_of(sizes[i]);
-        }
-        return i;
-    };
-    const auto groups = [&](const ClipArgs &a) {
-        return (int)hmax<int64_t>(1, hmin<int64_t>(a.chunks, (int64_t)kGroups * a.chunks / hmax<int64_t>(1, total)));
-    };
-    ClipArgs a{};
-    a.max_norm = max_norm;
-    a.eps = eps;
     int parts = 0;
+    Alone a{};
     for (int i = 0; i < count;) {
-        i = fill(a, i);
+        fill(a, i, count, in, nullptr, sizes, dtypes);
         if (!a.count) break;
         const int grid = groups(a);
         a.part = part + parts;
@@ -288,23 +316,10 @@ int stacr_clip_gradients(int count, const void *const *in, void *const *out, con
             else k_grad_norm<0><<<grid, kBlock, 0, s>>>(a);
         });
     }
-    a.part = part;
-    a.parts = parts;
-    a.norm_out = norm;
-    int i = 0;
-    do {
-        a.count = 0;
-        a.chunks = 0;
-        if (out) i = fill(a, i);
-        const int grid = a.count ? groups(a) : 1;
-        if (a.count || a.norm_out)
-            stacr_launch("k_grad_clip", s, [&] {
-                if (norm_type == 2) k_grad_clip<2><<<grid, kBlock, 0, s>>>(a);
-                else if (norm_type == 1) k_grad_clip<1><<<grid, kBlock, 0, s>>>(a);
-                else k_grad_clip<0><<<grid, kBlock, 0, s>>>(a);
-            });
-        a.norm_out = nullptr;
-    } while (out && i < count);
+    bool place = true;
+    for (int i = 0; out && i < count; ++i) place = place && out[i] == in[i];
+    if (place) clip_launches<Alone>(norm_type, count, in, out, sizes, dtypes, max_norm, eps, part, parts, norm, s);
+    else clip_launches<Pairs>(norm_type, count, in, out, sizes, dtypes, max_norm, eps, part, parts, norm, s);
     return stacr_hip_check(hipGetLastError(), "gradient clipping kernels");
 }
 

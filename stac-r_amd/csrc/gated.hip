@@ -496,8 +496,8 @@ __global__ __launch_bounds__(WM *WN * 64, 1) void k_gated_mm(const MmArgs p)
                                 float a[4], b[4];
                                 quad(acc[i][j + u], a);
                                 quad(acc[i][j + 2 + u], b);
-                                put_kept<DT>(u ? p.up : p.gate, u ? p.up_low : p.gate_low, m * p.ldo, lane, a, b, f0 + j * 8,
-                                             p.N, m < p.M);
+                                put_kept<DT>(u ? p.up : p.gate, u ? p.up_low : p.gate_low, m * p.ff_pad, lane, a, b, f0 + j * 8,
+                                             p.ff_pad, m < p.M);
                             }
                     }
                 }
@@ -564,12 +564,26 @@ __global__ __launch_bounds__(kBlock) void k_gated_join(const float *__restrict__
 
 // ------------------------------------------------------------------ operands that need another form
 // rows x cols of `src` (row stride ld) as rows of ld_dst (a multiple of 8, zeros past cols): fp32 as its
-// four bf16 planes, 16-bit types as they are
-template <int DT>
-__global__ __launch_bounds__(kBlock) void k_gated_pack(const void *__restrict__ src, int64_t ld, int64_t rows,
-                                                       int64_t cols, uint16_t *__restrict__ dst, int64_t ld_dst, bool vec)
+// four bf16 planes, 16-bit types as they are; up to three matrices a launch (grid.y)
+struct PackOne {
+    const void *src;
+    int64_t ld, rows;
+    uint16_t *dst;
+    bool vec;
+};
+struct PackArgs {
+    PackOne m[3];
+    int64_t cols, ld_dst;
+};
+
+template <int DT> __global__ __launch_bounds__(kBlock) void k_gated_pack(const PackArgs p)
 {
-    const int64_t chunks = ld_dst / 8, n = rows * chunks, plane = rows * ld_dst;
+    const PackOne o = p.m[blockIdx.y];
+    const void *__restrict__ src = o.src;
+    uint16_t *__restrict__ dst = o.dst;
+    const int64_t ld = o.ld, cols = p.cols, ld_dst = p.ld_dst;
+    const bool vec = o.vec;
+    const int64_t chunks = ld_dst / 8, n = o.rows * chunks, plane = o.rows * ld_dst;
     for (int64_t i = (int64_t)blockIdx.x * kBlock + threadIdx.x; i < n; i += (int64_t)gridDim.x * kBlock) {
         const int64_t row = i / chunks, c = (i - row * chunks) * 8;
         if constexpr (DT == STACR_DTYPE_F32) {
@@ -616,48 +630,42 @@ __global__ __launch_bounds__(kBlock) void k_gated_slopes(const void *__restrict_
     with_activation(act, [&](auto c) __attribute__((always_inline)) {
 #pragma unroll 2
         for (int64_t i = (int64_t)blockIdx.x * kBlock + threadIdx.x; i < n; i += (int64_t)gridDim.x * kBlock) {
-            const int64_t m = i / eighths, f = (i - m * eighths) * 8, at = m * ff + f;
-            const int have = ff - f < 8 ? (int)(ff - f) : 8;
+            const int64_t m = i / eighths, f = (i - m * eighths) * 8, at = m * ff_pad + f;
+            const int have = ff - f < 8 ? (int)(ff - f) : 8;  // outputs; the rest of the padded row gets zeros
             const auto read = [&](const void *src, const uint8_t *low, float(&v)[8]) __attribute__((always_inline)) {
                 if constexpr (EXACT) {
-                    const float *p = static_cast<const float *>(src) + at;
-                    if (have == 8) {
-                        __builtin_memcpy(v, p, 32);
-                    } else {
-#pragma unroll
-                        for (int k = 0; k < 8; ++k) v[k] = k < have ? p[k] : 0.0f;
-                    }
+                    __builtin_memcpy(v, static_cast<const float *>(src) + at, 32);
                 } else {
-                    const uint4 w = get8(static_cast<const T *>(src) + at, 0, have);
+                    const uint4 w = *reinterpret_cast<const uint4 *>(static_cast<const T *>(src) + at);
                     const uint32_t q[4] = {w.x, w.y, w.z, w.w};
                     uint2 b = make_uint2(0, 0);
-                    if (LOW && low) {
-                        if (have == 8) {
-                            __builtin_memcpy(&b, low + at, 8);
-                        } else {
-#pragma unroll
-                            for (int k = 0; k < 8; ++k)
-                                if (k < have) (k < 4 ? b.x : b.y) |= (uint32_t)low[at + k] << (k & 3) * 8;
-                        }
-                    }
+                    if constexpr (LOW) b = *reinterpret_cast<const uint2 *>(low + at);
 #pragma unroll
                     for (int k = 0; k < 8; ++k) {
                         const uint32_t h = q[k >> 1] >> (k & 1) * 16 & 0xffffu;
-                        if (LOW && low) v[k] = __uint_as_float(h << 16 | ((k < 4 ? b.x : b.y) >> (k & 3) * 8 & 255u) << 8);
+                        if constexpr (LOW) v[k] = __uint_as_float(h << 16 | ((k < 4 ? b.x : b.y) >> (k & 3) * 8 & 255u) << 8);
                         else v[k] = Act<DT>::ld((T)h);
                     }
                 }
             };
             float d[8], g[8], u[8], dg[8], du[8];
-            read(dh, nullptr, d);
+            if constexpr (EXACT) {
+#pragma unroll
+                for (int k = 0; k < 8; ++k) d[k] = k < have ? static_cast<const float *>(dh)[m * ff + f + k] : 0.0f;
+            } else {
+                const uint4 w = get8(static_cast<const T *>(dh) + m * ff + f, 0, have);
+                const uint32_t q[4] = {w.x, w.y, w.z, w.w};
+#pragma unroll
+                for (int k = 0; k < 8; ++k) d[k] = Act<DT>::ld((T)(q[k >> 1] >> (k & 1) * 16));
+            }
             read(gate, gate_low, g);
             read(up, up_low, u);
 #pragma unroll
             for (int k = 0; k < 8; ++k) {
                 float a, slope;
                 activate<EXACT, decltype(c)::value>(g[k], a, slope);
-                dg[k] = d[k] * u[k] * slope;
-                du[k] = d[k] * a;
+                dg[k] = k < have ? d[k] * u[k] * slope : 0.0f;
+                du[k] = k < have ? d[k] * a : 0.0f;
             }
             uint16_t *row = dgu + m * 2 * ff_pad + f;
 #pragma unroll
@@ -855,7 +863,7 @@ __global__ __launch_bounds__(kBlock) void k_gated_few(const FewArgs p)
         activate<DT == STACR_DTYPE_F32>(p.act, g, a, slope);
         store_any(p.h, DT, m * p.ff + ff, a * u);
         if (p.gate) {
-            const int64_t at = m * p.ff + ff;
+            const int64_t at = m * ((p.ff + 7) & ~7ll) + ff;
             if (DT != STACR_DTYPE_F32 && p.gate_low) {
                 const uint32_t x = to_24(g), y = to_24(u);
                 static_cast<uint16_t *>(p.gate)[at] = (uint16_t)(x >> 16);
@@ -925,11 +933,11 @@ void mm_run(MmArgs p, int a_cu, hipStream_t s)
 int64_t tiles(int64_t m, int64_t n, int bm, int bn) { return ((m + bm - 1) / bm) * ((n + bn - 1) / bn); }
 
 // The tile of a product and how many workgroups share its K, by what they cost, in steps of a 256 x 256
-// tile (1.7 us): a round is as many tiles as the chip holds at once, a tile costs its steps and about 3 more
+// tile (1.7 us): a round is as many tiles as the chip holds at once, a tile costs its steps and about 6 more
 // for its start and its results; partial products are written and read again (8192 x 1024 in two: 20 us).
 //   256 x 256   8 waves, one workgroup a CU: 1 a step
 //   256 x 128   8 waves, one workgroup a CU: 0.66 for half the work (LDS and L2 move 1.5 times as much for it)
-//   128 x 128   4 waves, two workgroups a CU: 0.62 for both, half the work together
+//   128 x 128   4 waves, two workgroups a CU: 0.6 for both, half the work together
 // (8192 x 1024 of K 8192, 128 tiles of 256 x 256: 130 us and 20 to join two splits; 256 of 256 x 128: 150 us;
 // 512 of 128 x 128: 130 to 142 us.)
 struct ProductPlan {
@@ -939,7 +947,7 @@ struct ProductPlan {
 ProductPlan product_plan(int64_t m, int64_t n, int halves, int64_t k, int nseg, bool dual)
 {
     const int64_t steps = hmax<int64_t>(1, (k + kMmK - 1) / kMmK * nseg);
-    const double cost[3] = {1.0, 0.66, 0.62};
+    const double cost[3] = {1.0, 0.66, 0.6};
     const int bm[3] = {256, 256, 128}, bn[3] = {256, 128, 128}, slots[3] = {kCus, kCus, 2 * kCus};
     ProductPlan best{0, 1};
     double least = 1e300;
@@ -947,7 +955,7 @@ ProductPlan product_plan(int64_t m, int64_t n, int halves, int64_t k, int nseg, 
         const int64_t each = tiles(m, n, bm[t], dual ? bn[t] / 2 : bn[t]) * halves;
         for (int s = 1; s <= (dual ? 1 : 16) && s * 4 <= steps + 3; ++s) {
             const int64_t rounds = (each * s + slots[t] - 1) / slots[t];
-            double c = rounds * ((double)((steps + s - 1) / s) + 3.0) * cost[t];
+            double c = rounds * ((double)((steps + s - 1) / s) + 6.0) * cost[t];
             if (s > 1) c += 2.5 + (double)m * n * halves * 8.0 * s / 7.0e6 / 1.7;
             if (c < least) least = c, best = ProductPlan{t, s};
         }
@@ -1007,18 +1015,6 @@ Pieces pieces(const Problem &q, bool backward)
 
 int blocks_for(int64_t n) { return (int)hmin<int64_t>((n + kBlock - 1) / kBlock, 4096); }
 
-void pack(int dt, const void *src, int64_t ld, int64_t rows, int64_t cols, uint16_t *dst, int64_t ld_dst, hipStream_t s)
-{
-    const int64_t n = rows * ld_dst / 8;
-    if (n == 0) return;
-    const bool vec = aligned_to(src, 16) && ld % 4 == 0;
-    stacr_launch("k_gated_pack", s, [&] {
-        if (dt == STACR_DTYPE_F32)
-            k_gated_pack<STACR_DTYPE_F32><<<blocks_for(n), kBlock, 0, s>>>(src, ld, rows, cols, dst, ld_dst, vec);
-        else k_gated_pack<STACR_DTYPE_BF16><<<blocks_for(n), kBlock, 0, s>>>(src, ld, rows, cols, dst, ld_dst, false);
-    });
-}
-
 template <int DT, int NT> void few_launch(const FewArgs &a, bool vec, hipStream_t s)
 {
     const int grid = (int)((a.ff + 15) / 16);
@@ -1051,22 +1047,34 @@ Operands operands(const Problem &q, const void *x, const void *wg, const void *w
     o.wu = static_cast<const uint16_t *>(wu);
     o.x_ld = q.x_ld;
     o.w_ld = q.d;
+    PackArgs a{};
+    a.cols = q.d;
+    a.ld_dst = q.d_pad;
+    int count = 0;
+    int64_t most = 0;
+    const auto pack = [&](const void *src, int64_t ld, int64_t rows, size_t at) {
+        uint16_t *dst = reinterpret_cast<uint16_t *>(ws + at);
+        a.m[count++] = PackOne{src, ld, rows, dst, aligned_to(src, 16) && ld % 4 == 0};
+        most = hmax(most, rows * q.d_pad / 8);
+        return dst;
+    };
     if (q.pack_x && need_x) {
-        uint16_t *dst = reinterpret_cast<uint16_t *>(ws + w.x);
-        pack(q.dt, x, q.x_ld, q.rows, q.d, dst, q.d_pad, s);
-        o.x = dst;
+        o.x = pack(x, q.x_ld, q.rows, w.x);
         o.x_ld = q.d_pad;
         o.x_plane = (size_t)q.rows * q.d_pad;
     }
     if (q.pack_w && need_w) {
-        uint16_t *g = reinterpret_cast<uint16_t *>(ws + w.wg), *u = reinterpret_cast<uint16_t *>(ws + w.wu);
-        pack(q.dt, wg, q.d, q.ff, q.d, g, q.d_pad, s);
-        pack(q.dt, wu, q.d, q.ff, q.d, u, q.d_pad, s);
-        o.wg = g;
-        o.wu = u;
+        o.wg = pack(wg, q.d, q.ff, w.wg);
+        o.wu = pack(wu, q.d, q.ff, w.wu);
         o.w_ld = q.d_pad;
         o.w_plane = (size_t)q.ff * q.d_pad;
     }
+    if (count)
+        stacr_launch("k_gated_pack", s, [&] {
+            const dim3 grid((unsigned)blocks_for(most), (unsigned)count);
+            if (q.dt == STACR_DTYPE_F32) k_gated_pack<STACR_DTYPE_F32><<<grid, kBlock, 0, s>>>(a);
+            else k_gated_pack<STACR_DTYPE_BF16><<<grid, kBlock, 0, s>>>(a);
+        });
     return o;
 }
 
@@ -1153,6 +1161,8 @@ int check_kept(const char *what, int dtype, const void *gate, const void *up, co
 {
     if ((gate == nullptr) != (up == nullptr) || (gate_low == nullptr) != (up_low == nullptr) || (gate_low && !gate))
         return stacr_fail(STACR_ERR_INVALID, "%s: gate goes with up, gate_low with up_low, both with gate and up", what);
+    if (!aligned_to(gate, 16) || !aligned_to(up, 16) || !aligned_to(gate_low, 16) || !aligned_to(up_low, 16))
+        return stacr_fail(STACR_ERR_INVALID, "%s: kept pre-activations must be 16-byte aligned", what);
     if (gate_low && dtype == STACR_DTYPE_F32)
         return stacr_fail(STACR_ERR_INVALID, "%s: fp32 pre-activations have no low bytes", what);
     return STACR_OK;

@@ -617,9 +617,10 @@ def gated_forward(x2d: torch.Tensor, w_gate: torch.Tensor, w_up: torch.Tensor, b
     h = x2d.new_empty((rows, ff))
     gate = up = gate_low = up_low = None
     if keep is not None:
-        gate, up = torch.empty_like(h), torch.empty_like(h)
+        shape = (rows, (ff + 7) // 8 * 8)  # rows padded to whole pieces of 8
+        gate, up = h.new_empty(shape), h.new_empty(shape)
         if keep == "full" and code != _lib.DTYPE_F32:
-            gate_low, up_low = (torch.empty((rows, ff), dtype=torch.uint8, device=h.device) for _ in range(2))
+            gate_low, up_low = h.new_empty(shape, dtype=torch.uint8), h.new_empty(shape, dtype=torch.uint8)
     ws, nbytes = (None, 0) if rows <= GATED_FEW_ROWS else _gated_workspace(x2d, code, rows, d, x_ld, w_gate, w_up, 0)
     rc = _lib.load().stacr_gated_forward(x2d.data_ptr(), code, rows, d, x_ld, w_gate.data_ptr(), w_up.data_ptr(), ff,
                                          _at(b_gate), _at(b_up), _lib.ACTIVATION_CODES[activation], h.data_ptr(),

@@ -283,7 +283,7 @@ def test_kept_preactivations(dev, rows, d, ff, dtype):
     g = kept[0]
     assert torch.equal(h, kernels.gated_forward(x, wg, wu, bg, bu, "silu"))
     g64 = x.double() @ wg.double().t() + bg.double()
-    assert off(g, g64) <= tolerance(dtype, d, False)
+    assert off(g[:, :ff], g64) <= tolerance(dtype, d, False)
     give = dtype != "f32"
     dx, dwg, dwu, dbg, dbu, dgu = kernels.gated_backward(dh, x, wg, wu, bg, bu, "silu", kept=kept,
                                                          needs=(True, True, True, True), slopes=give)
