@@ -524,8 +524,8 @@ int stacr_gated_forward(const void *x, int dtype, int64_t rows, int64_t d, int64
  * both NULL: g and u are then computed again from x and the weights, so that a caller keeps nothing but x.
  * Each of dx, (dw_gate, dw_up), db_gate, db_up may be NULL.  x may be NULL when gate and up are given and
  * no weight gradient is asked for; the weights may be when dx is not either.  dg and du are rounded to
- * the type before the products.  dgu (16-bit types; NULL: kept in the workspace) receives [dg | du], rows
- * x 2 p with p = ff rounded up to 8 and zeros past ff: the gradient that a weight-gradient call on x's
+ * the type before the products.  dgu (16-byte aligned; fp32: only with gate and up; NULL: kept in the
+ * workspace) receives [dg | du], rows x 2 p with p = ff rounded up to 8 and zeros past ff: the gradient that a weight-gradient call on x's
  * saved factors takes for both projections at once.
  */
 int stacr_gated_backward(const void *dh, const void *x, int dtype, int64_t rows, int64_t d, int64_t x_ld,

@@ -617,12 +617,14 @@ template <int DT> __global__ __launch_bounds__(kBlock) void k_gated_pack(const P
 }
 
 // ------------------------------------------------------------------ kept pre-activations
-// [dg | du] from dh and the kept g and u, eight values a thread; LOW: g and u in 24 bits
+// [dg | du] from dh and the kept g and u, eight values a thread; LOW: g and u in 24 bits; plain: fp32
+// values beside their planes, or NULL
 template <int DT, bool LOW>
 __global__ __launch_bounds__(kBlock) void k_gated_slopes(const void *__restrict__ dh, const void *__restrict__ gate,
                                                          const void *__restrict__ up, const uint8_t *__restrict__ gate_low,
                                                          const uint8_t *__restrict__ up_low, int64_t rows, int64_t ff, int act,
-                                                         uint16_t *__restrict__ dgu, int64_t ff_pad, int64_t plane)
+                                                         uint16_t *__restrict__ dgu, int64_t ff_pad, int64_t plane,
+                                                         float *__restrict__ plain)
 {
     using T = typename Act<DT>::T;
     constexpr bool EXACT = DT == STACR_DTYPE_F32;
@@ -673,6 +675,7 @@ __global__ __launch_bounds__(kBlock) void k_gated_slopes(const void *__restrict_
                 const float(&v)[8] = half ? du : dg;
                 uint16_t *o = row + half * ff_pad;
                 if constexpr (EXACT) {
+                    if (plain) __builtin_memcpy(plain + (m * 2 + half) * ff_pad + f, v, 32);
                     uint16_t s[8][kPlanes];
 #pragma unroll
                     for (int k = 0; k < 8; ++k) split_f32(v[k], s[k]);
@@ -1134,12 +1137,12 @@ void product_typed(int dt, MmArgs p, const ProductPlan &plan, float *part, hipSt
 
 template <int DT>
 void slopes_launch(const void *dh, const void *gate, const void *up, const uint8_t *gate_low, const uint8_t *up_low,
-                   const Problem &q, int act, uint16_t *dgu, int64_t plane, hipStream_t s)
+                   const Problem &q, int act, uint16_t *dgu, int64_t plane, float *plain, hipStream_t s)
 {
     const int grid = blocks_for(q.rows * q.ff_pad / 8);
     stacr_launch("k_gated_slopes", s, [&] {
-        if (gate_low) k_gated_slopes<DT, true><<<grid, kBlock, 0, s>>>(dh, gate, up, gate_low, up_low, q.rows, q.ff, act, dgu, q.ff_pad, plane);
-        else k_gated_slopes<DT, false><<<grid, kBlock, 0, s>>>(dh, gate, up, nullptr, nullptr, q.rows, q.ff, act, dgu, q.ff_pad, plane);
+        if (gate_low) k_gated_slopes<DT, true><<<grid, kBlock, 0, s>>>(dh, gate, up, gate_low, up_low, q.rows, q.ff, act, dgu, q.ff_pad, plane, plain);
+        else k_gated_slopes<DT, false><<<grid, kBlock, 0, s>>>(dh, gate, up, nullptr, nullptr, q.rows, q.ff, act, dgu, q.ff_pad, plane, plain);
     });
 }
 
@@ -1249,8 +1252,8 @@ int stacr_gated_backward(const void *dh, const void *x, int dtype, int64_t rows,
     if (bad) return bad;
     if (rows && (!dh || (!x && (!kept || weights)) || ((!w_gate || !w_up) && (!kept || dx))))
         return stacr_fail(STACR_ERR_INVALID, "stacr_gated_backward: NULL pointer argument");
-    if (dgu && dtype == STACR_DTYPE_F32)
-        return stacr_fail(STACR_ERR_UNSUPPORTED, "stacr_gated_backward: [dg | du] is given out for 16-bit types only");
+    if (dgu && dtype == STACR_DTYPE_F32 && !kept)
+        return stacr_fail(STACR_ERR_UNSUPPORTED, "stacr_gated_backward: fp32 [dg | du] is given out from gate and up only");
     if (dgu && !aligned_to(dgu, 16))
         return stacr_fail(STACR_ERR_INVALID, "stacr_gated_backward: [dg | du] must be 16-byte aligned");
     hipStream_t s = static_cast<hipStream_t>(stream);
@@ -1261,14 +1264,16 @@ int stacr_gated_backward(const void *dh, const void *x, int dtype, int64_t rows,
                           w.total);
     char *ws = static_cast<char *>(workspace);
     const int64_t plane = rows * 2 * q.ff_pad;
-    uint16_t *slopes = dgu ? static_cast<uint16_t *>(dgu) : reinterpret_cast<uint16_t *>(ws + w.dgu);
+    // fp32's planes are the workspace's, its values go out beside them
+    float *plain = dtype == STACR_DTYPE_F32 ? static_cast<float *>(dgu) : nullptr;
+    uint16_t *slopes = dgu && !plain ? static_cast<uint16_t *>(dgu) : reinterpret_cast<uint16_t *>(ws + w.dgu);
     float *part = reinterpret_cast<float *>(ws + w.part);
     const Operands o = operands(q, x, w_gate, w_up, ws, w, rows > 0 && (!kept || weights), rows > 0 && (!kept || dx), s);
     if (rows && kept) {
         const uint8_t *gl = static_cast<const uint8_t *>(gate_low), *ul = static_cast<const uint8_t *>(up_low);
-        if (dtype == STACR_DTYPE_F32) slopes_launch<STACR_DTYPE_F32>(dh, gate, up, nullptr, nullptr, q, activation, slopes, plane, s);
-        else if (dtype == STACR_DTYPE_BF16) slopes_launch<STACR_DTYPE_BF16>(dh, gate, up, gl, ul, q, activation, slopes, plane, s);
-        else slopes_launch<STACR_DTYPE_F16>(dh, gate, up, gl, ul, q, activation, slopes, plane, s);
+        if (dtype == STACR_DTYPE_F32) slopes_launch<STACR_DTYPE_F32>(dh, gate, up, nullptr, nullptr, q, activation, slopes, plane, plain, s);
+        else if (dtype == STACR_DTYPE_BF16) slopes_launch<STACR_DTYPE_BF16>(dh, gate, up, gl, ul, q, activation, slopes, plane, nullptr, s);
+        else slopes_launch<STACR_DTYPE_F16>(dh, gate, up, gl, ul, q, activation, slopes, plane, nullptr, s);
     } else if (rows) {
         MmArgs p = gated_args(q, o, b_gate, b_up, activation);
         p.dh = dh;

@@ -7,7 +7,7 @@ include/stacr_amd.h); this package is the host side.
 from .adaptive import AdaptiveSTACRConfig, AdaptiveSTACRLinear, apply_adaptive_stacr, set_stacr_runtime_state
 from .clip import clip_grad_norm, clip_gradients, grad_norm
 from .compressor import STACRCompressor, STACRConfig, stacr_saved_tensors
-from .gated import gated_feed_forward
+from .gated import STACRGatedFeedForward, gated_feed_forward
 from .layers import STACRFunction, STACRLinear
 from .memory import saved_surface_predictor, stacr_stored_bytes
 from .quant import QuantizedValues, quantize_values
@@ -33,6 +33,7 @@ __all__ = [
     "apply_adaptive_stacr",
     "set_stacr_runtime_state",
     "gated_feed_forward",
+    "STACRGatedFeedForward",
     "rotary",
     "rotary_tables",
     "clip_gradients",

@@ -1,15 +1,18 @@
 """The gated feed-forward block h = act(x Wg^T + bg) * (x Wu^T + bu) and its gradients in HIP kernels.
 
 ``gated_feed_forward`` is the exact operator: one kernel forms both projections, the activation and the
-product.
+product.  ``STACRGatedFeedForward`` is the block with its input compressed as STACRLinear compresses it: one
+save serves both projections, whose weight gradients come from one call on [dg | du].
 (No counterpart in the reference, whose layers wrap the projections one by one.)
 """
 from __future__ import annotations
 
 import torch
+from torch import nn
 from torch.autograd.function import once_differentiable
 
 from . import _lib, kernels
+from .layers import STACRLinear, _save_factors
 
 ACTIVATIONS = tuple(_lib.ACTIVATION_CODES)
 
@@ -102,4 +105,102 @@ def gated_feed_forward(x: torch.Tensor, w_gate: torch.Tensor, w_up: torch.Tensor
     return h.view(*x.shape[:-1], h.shape[1])
 
 
-__all__ = ["ACTIVATIONS", "GatedFeedForwardFunction", "gated_feed_forward"]
+class STACRGatedFunction(torch.autograd.Function):
+    """Exact forward and input gradient; weight gradients from the input's saved factors.
+
+    Saved tensors: both weights and biases, coefficients, basis, the residual's indices, values and scale,
+    and the two pre-activations in the type (the input itself is not kept, so they cannot be formed again).
+    """
+
+    @staticmethod
+    def forward(ctx, x, w_gate, w_up, b_gate, b_up, basis, budget, bits, chunk_rows, mode, block_size, sample_ratio,
+                activation):
+        x2d = x.reshape(-1, x.shape[-1])
+        h, kept = kernels.gated_forward(x2d, w_gate, w_up, _contiguous(b_gate), _contiguous(b_up), activation, "type")
+        if mode == "none":
+            mode, budget = "chunk_topk", 0.0
+        coeff, idx, data, scale, census, bits, _ = _save_factors(x2d, basis.to(x.dtype), mode, float(budget), int(bits),
+                                                                 int(chunk_rows), int(block_size), float(sample_ratio))
+        ctx.save_for_backward(w_gate, w_up, b_gate, b_up, coeff, basis.to(x.dtype), idx, data, scale, kept[0], kept[1])
+        # the save's entry census (an intermediate, outside the saved tensors): the weight gradient need not count
+        ctx.census = census if idx is not None else None
+        ctx.bits, ctx.shape, ctx.activation = bits if idx is not None else 0, x.shape, activation
+        return h.view(*x.shape[:-1], h.shape[1])
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, dh):
+        w_gate, w_up, b_gate, b_up, coeff, q, idx, data, scale, gate, up = ctx.saved_tensors
+        need = ctx.needs_input_grad
+        weights = need[1] or need[2]
+        with torch.autocast(device_type=dh.device.type, enabled=False):
+            dx, _, _, dbg, dbu, dgu = kernels.gated_backward(
+                dh.reshape(-1, dh.shape[-1]), None, w_gate, w_up, _contiguous(b_gate), _contiguous(b_up), ctx.activation,
+                (gate, up, None, None), (need[0], False, need[3], need[4]), slopes=weights)
+            dwg = dwu = None
+            if weights:
+                residual = (idx, data, scale) if idx is not None and idx.numel() else None
+                dw, _ = kernels.weight_grad(dgu, coeff, q, residual, ctx.bits, False, w_gate.dtype, census=ctx.census)
+                ff, pad = w_gate.shape[0], dgu.shape[1] // 2
+                dwg, dwu = dw[:ff] if need[1] else None, dw[pad:pad + ff] if need[2] else None
+        return (dx.view(ctx.shape) if dx is not None else None, dwg, dwu, dbg, dbu) + (None,) * 8
+
+
+class STACRGatedFeedForward(nn.Module):
+    """act(gate(x)) * up(x) of two projections of one input, whose saved copy is compressed once for both.
+
+    ``gate`` holds the gate projection's parameters and the basis with its schedule (a STACRLinear: set_step on
+    a model reaches it); the up projection's are ``up_weight`` and ``up_bias``.  Options as STACRLinear's.
+    Eval, no-grad and frozen-weight calls run gated_feed_forward, as do inputs without rows.
+    """
+
+    def __init__(self, gate: STACRLinear, up_weight: nn.Parameter, up_bias: nn.Parameter | None, *,
+                 activation: str = "silu"):
+        super().__init__()
+        if activation not in _lib.ACTIVATION_CODES:
+            raise ValueError(f"activation must be one of {list(ACTIVATIONS)}, got {activation!r}")
+        if gate.transposed:
+            raise ValueError("the gate projection must keep its weight as (out, in)")
+        if up_weight.shape != gate.weight.shape or up_weight.dtype != gate.weight.dtype:
+            raise ValueError(f"gate and up weights differ: {tuple(gate.weight.shape)} {gate.weight.dtype} and "
+                             f"{tuple(up_weight.shape)} {up_weight.dtype}")
+        if up_bias is not None and up_bias.shape != up_weight.shape[:1]:
+            raise ValueError("bias shape must match the output feature count")
+        self.gate, self.up_weight, self.up_bias, self.activation = gate, up_weight, up_bias, activation
+        self.in_features, self.out_features = gate.in_features, gate.out_features
+
+    @classmethod
+    def from_linears(cls, gate: nn.Linear, up: nn.Linear, *, activation: str = "silu", **options) -> "STACRGatedFeedForward":
+        """The block of two nn.Linear layers, whose parameters it takes over."""
+        if not (isinstance(gate, nn.Linear) and isinstance(up, nn.Linear)):
+            raise TypeError("from_linears requires two nn.Linear layers")
+        block = cls(STACRLinear.from_linear(gate, **options), up.weight, up.bias, activation=activation)
+        return block.train(gate.training)
+
+    def forward(self, x: torch.Tensor) -> torch.Tensor:
+        if x.ndim < 1 or x.shape[-1] != self.in_features:
+            raise ValueError(f"Expected last input dimension {self.in_features}, got {tuple(x.shape)}")
+        gate = self.gate
+        w = [gate.weight, self.up_weight, gate.bias, self.up_bias]
+        if not (self.training and torch.is_grad_enabled() and x.numel() > 0 and
+                (gate.weight.requires_grad or self.up_weight.requires_grad)):
+            return gated_feed_forward(x, *w, activation=self.activation)
+        if torch.is_autocast_enabled(x.device.type):
+            dtype = torch.get_autocast_dtype(x.device.type)
+            x, *w = (None if t is None else t.to(dtype) for t in (x, *w))
+        _check_gated(x, *w, self.activation)
+        basis, budget = gate._factor_state(x)
+        with torch.autocast(device_type=x.device.type, enabled=False):
+            return STACRGatedFunction.apply(x, *w, basis, budget, gate.residual_bits, gate.chunk_rows, gate.residual_mode,
+                                            gate.residual_block_size, gate.residual_sample_ratio, self.activation)
+
+    def stored_bytes(self, rows: int, value_bytes: int = 2) -> dict:
+        """STACRLinear.stored_bytes of the shared input, and the kept pre-activations."""
+        stored = self.gate.stored_bytes(rows, value_bytes)
+        stored["preactivations"] = 2 * int(rows) * ((self.out_features + 7) // 8 * 8) * value_bytes
+        stored["total"] += stored["preactivations"]
+        return stored
+
+
+__all__ = ["ACTIVATIONS", "GatedFeedForwardFunction", "STACRGatedFeedForward", "STACRGatedFunction",
+           "gated_feed_forward"]

@@ -637,7 +637,7 @@ def gated_backward(dh: torch.Tensor, x2d: torch.Tensor | None, w_gate: torch.Ten
     """(dx, dw_gate, dw_up, db_gate, db_up, dgu) for dh, None where ``needs`` (input, weights, gate bias, up
     bias) asks for none (stacr_gated_backward).  ``kept``: what gated_forward kept, or None to compute it
     again from x2d, which may be None with them when no weight gradient is asked for.  ``slopes``: give
-    out dgu = [dg | du], rows x 2 p with p = ff rounded up to 8 (16-bit types)."""
+    out dgu = [dg | du], rows x 2 p with p = ff rounded up to 8 (float32: only with ``kept``)."""
     dh, w_gate, w_up = dh.contiguous(), w_gate.contiguous(), w_up.contiguous()
     rows, ff = dh.shape
     d = w_gate.shape[1]

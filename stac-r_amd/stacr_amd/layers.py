@@ -63,6 +63,25 @@ def _select_residual(x, coeff, basis, budget, chunk_rows, mode, block_size=16, s
     return kernels.select_sampled(x, coeff, q, float(budget), float(sample_ratio), k_total)
 
 
+def _save_factors(activation, q, mode, budget, bits, chunk_rows, block_size, sample_ratio):
+    """(coeff, idx, data, scale, census, bits, length) of one save of the rows of ``activation`` on the basis
+    ``q`` in its dtype; idx, data and scale are None without a residual."""
+    census = None
+    if mode in TOPK_SELECTORS or (mode == "block_sparse" and activation.shape[1] % block_size):
+        # projection, selection and quantization in one stacr_save call
+        sel = "global_topk" if mode == "global_topk" else "chunk_topk"
+        coeff, idx, data, scale, census = kernels.save_with_census(activation, q, mode=sel, budget=budget,
+                                                                   chunk_rows=chunk_rows, bits=bits)
+        return coeff, idx, data, scale, census, bits, int(idx.numel()) if idx is not None else 0
+    # projection, then the selector's kernels, then quantize_values
+    coeff, _, _, _ = kernels.save(activation, q, mode="chunk_topk", budget=0.0, chunk_rows=chunk_rows, bits=0)
+    idx, val = _select_residual(activation, coeff, q, budget, chunk_rows, mode, block_size, sample_ratio)
+    if idx is None:
+        return coeff, None, None, None, None, bits, 0
+    packed = quantize_values(val, bits)
+    return coeff, idx, packed.data, packed.scale, None, packed.bits, packed.length
+
+
 class STACRFunction(torch.autograd.Function):
     """Exact linear forward and input gradient; weight gradient from the saved factors.
 
@@ -87,22 +106,8 @@ class STACRFunction(torch.autograd.Function):
             mode, budget = "chunk_topk", 0.0
         with torch.autocast(device_type=x.device.type, enabled=False):
             activation, q = x2d.to(out2d.dtype), basis.to(out2d.dtype)
-            fused = mode in TOPK_SELECTORS or (mode == "block_sparse" and d_in % int(residual_block_size))
-            census = None
-            if fused:  # projection, selection and quantization in one stacr_save call
-                sel = "global_topk" if mode == "global_topk" else "chunk_topk"
-                coeff, idx, data, scale, census = kernels.save_with_census(activation, q, mode=sel, budget=budget,
-                                                                           chunk_rows=int(chunk_rows), bits=bits)
-                length = int(idx.numel()) if idx is not None else 0
-            else:  # projection, then the selector's kernels, then quantize_values
-                coeff, _, _, _ = kernels.save(activation, q, mode="chunk_topk", budget=0.0,
-                                              chunk_rows=int(chunk_rows), bits=0)
-                idx, val = _select_residual(activation, coeff, q, budget, int(chunk_rows), mode,
-                                            int(residual_block_size), float(residual_sample_ratio))
-                data = scale = None
-                if idx is not None:
-                    packed = quantize_values(val, bits)
-                    data, scale, bits, length = packed.data, packed.scale, packed.bits, packed.length
+            coeff, idx, data, scale, census, bits, length = _save_factors(
+                activation, q, mode, budget, bits, int(chunk_rows), int(residual_block_size), float(residual_sample_ratio))
         saved = [coeff, weight, q]
         if idx is not None:
             saved += [idx, data, scale]

@@ -284,19 +284,19 @@ def test_kept_preactivations(dev, rows, d, ff, dtype):
     assert torch.equal(h, kernels.gated_forward(x, wg, wu, bg, bu, "silu"))
     g64 = x.double() @ wg.double().t() + bg.double()
     assert off(g[:, :ff], g64) <= tolerance(dtype, d, False)
-    give = dtype != "f32"
+    half = dtype != "f32"
     dx, dwg, dwu, dbg, dbu, dgu = kernels.gated_backward(dh, x, wg, wu, bg, bu, "silu", kept=kept,
-                                                         needs=(True, True, True, True), slopes=give)
+                                                         needs=(True, True, True, True), slopes=True)
     _, want = formula([x, wg, wu, bg, bu], dh, "silu")
-    room = 1.5 if give else 1.0
+    room = 1.5 if half else 1.0
     for a, b in zip((dx, dwg, dwu, dbg, dbu), want):
         assert off(a, b) <= room * tolerance(dtype, max(rows, d, ff), True)
-    if give:
-        pad = (ff + 7) // 8 * 8
-        assert dgu.shape == (rows, 2 * pad) and not dgu[:, ff:pad].any() and not dgu[:, pad + ff:].any()
-        alone = kernels.gated_backward(dh, None, wg, wu, bg, bu, "silu", kept=kept, needs=(True, False, False, False),
-                                       slopes=True)
-        assert torch.equal(alone[0], dx) and torch.equal(alone[5], dgu)
+    pad = (ff + 7) // 8 * 8
+    assert dgu.shape == (rows, 2 * pad) and not dgu[:, ff:pad].any() and not dgu[:, pad + ff:].any()
+    assert off(dgu[:, :ff].double().t() @ x.double(), want[1]) <= room * tolerance(dtype, max(rows, d, ff), True)
+    alone = kernels.gated_backward(dh, None, wg, wu, bg, bu, "silu", kept=kept, needs=(True, False, False, False),
+                                   slopes=True)
+    assert torch.equal(alone[0], dx) and torch.equal(alone[5], dgu)
 
 
 def test_refusals(dev):
