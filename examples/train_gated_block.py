@@ -83,7 +83,7 @@ def train(steps: int = 200, batch: int = 64, length: int = 64, vocab: int = 64, 
         optimizer.step()
         losses.append(loss.detach())
         if report and (step + 1) % report == 0:
-            print(f"step {step + 1}: loss {float(loss):.3f}, gradient norm {float(norms[-1]):.3f}", flush=True)
+            print(f"step {step + 1}: loss {float(losses[-1]):.3f}, gradient norm {float(norms[-1]):.3f}", flush=True)
     return [float(v) for v in losses], [float(v) for v in norms]
 
 

@@ -86,6 +86,25 @@ __device__ __forceinline__ void load_vec(const typename Act<DT>::T *__restrict__
     }
 }
 
+// 16 bytes at p, at the alignment of 16-bit elements or more, past the caches' own order of use
+// (nontemporal): for streams that nothing reads again before they would be displaced.
+template <typename T> __device__ __forceinline__ uint4 load16_stream(const T *p)
+{
+    typedef uint32_t v4 __attribute__((ext_vector_type(4), aligned(2)));
+    const v4 w = __builtin_nontemporal_load(reinterpret_cast<const v4 *>(p));
+    return make_uint4(w.x, w.y, w.z, w.w);
+}
+
+template <typename T> __device__ __forceinline__ void store16_stream(T *p, uint4 v)
+{
+    typedef uint32_t v4 __attribute__((ext_vector_type(4), aligned(2)));
+    const v4 w = {v.x, v.y, v.z, v.w};
+    __builtin_nontemporal_store(w, reinterpret_cast<v4 *>(p));
+}
+
+// Bytes that the last-level cache (256 MB) holds: streams past it are better kept out of it.
+constexpr int64_t kCacheBytes = (int64_t)256 << 20;
+
 __device__ __forceinline__ float load_any(const void *p, int dt, int64_t i)
 {
     if (dt == STACR_DTYPE_F32) return static_cast<const float *>(p)[i];
