@@ -82,8 +82,9 @@ template <bool EXACT, int ACT> __device__ __forceinline__ void activate(float g,
         const float in = 0.79788456080286536f * (g + 0.044715f * g * g * g);
         const float t = 1.0f - 2.0f * inverse<EXACT>(1.0f + exp_of<EXACT>(2.0f * in));
         a = 0.5f * g * (1.0f + t);
-        slope = 0.5f * (1.0f + t) +
-                0.5f * g * (1.0f - t * t) * 0.79788456080286536f * (1.0f + 3.0f * 0.044715f * g * g);
+        const float bend = 1.0f - t * t;  // 0 in the tails, where g * g may be infinite
+        slope = 0.5f * (1.0f + t);
+        if (bend > 0.0f) slope += 0.5f * g * bend * 0.79788456080286536f * (1.0f + 3.0f * 0.044715f * g * g);
     } else if constexpr (ACT == STACR_ACT_RELU) {
         a = g > 0.0f ? g : (g != g ? g : 0.0f);
         slope = g > 0.0f ? 1.0f : 0.0f;
@@ -1200,7 +1201,7 @@ int check_problem(const char *what, int dtype, int64_t rows, int64_t d, int64_t 
     if (d > kMaxFeatures || ff > kMaxFeatures || x_ld > kMaxFeatures || rows >= (int64_t)1 << 24)
         return stacr_fail(STACR_ERR_UNSUPPORTED, "%s: more than 2^20 features, or 2^24 rows", what);
     // the products' grids, and the bias partials' second grid dimension
-    if (tiles(rows, ff, 128, 64) >= (int64_t)1 << 30)
+    if (tiles(rows, ff, 128, 64) >= (int64_t)1 << 30 || tiles(rows, d, 128, 128) >= (int64_t)1 << 30)
         return stacr_fail(STACR_ERR_UNSUPPORTED, "%s: more than 2^30 tiles", what);
     return STACR_OK;
 }

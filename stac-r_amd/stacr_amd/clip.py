@@ -69,8 +69,9 @@ def clip_gradients(grads: Iterable[torch.Tensor], max_norm: float, *, norm_type:
     their device.
 
     The norm is over all elements of all tensors (``norm_type`` 1, 2 or infinity) in 64 bits; types may
-    be mixed.  In place, or into the tensors of ``out`` (one of the same shape and type for each).  Nothing waits for the
-    GPU unless ``error_if_nonfinite`` asks whether the norm is finite, before anything is scaled.
+    be mixed.  In place, or into the tensors of ``out`` (for each gradient one of its type, and of its shape
+    or, all being contiguous, its number of elements).  Nothing waits for the GPU unless
+    ``error_if_nonfinite`` asks whether the norm is finite, before anything is scaled.
     """
     grads = list(grads)
     code = _norm_code(norm_type)
@@ -87,14 +88,14 @@ def clip_gradients(grads: Iterable[torch.Tensor], max_norm: float, *, norm_type:
     device = grads[0].device
     into, copies = at, []
     if out is not None:
-        into, _, out_codes, out_plain = _facts(out, "outputs")
+        into, out_sizes, out_codes, out_plain = _facts(out, "outputs")
         if out[0].device != device:
             raise RuntimeError(f"gradients are on {device}, outputs on {out[0].device}")
-        if codes != out_codes or [g.shape for g in grads] != [o.shape for o in out]:
-            for g, o in zip(grads, out):
-                if g.shape != o.shape or g.dtype != o.dtype:
-                    raise ValueError(f"an output of {tuple(o.shape)} {o.dtype} for a gradient of {tuple(g.shape)} {g.dtype}")
         plain = plain or out_plain
+        if codes != out_codes or sizes != out_sizes or (plain and [g.shape for g in grads] != [o.shape for o in out]):
+            for g, o in zip(grads, out):
+                if g.numel() != o.numel() or g.dtype != o.dtype or (plain and g.shape != o.shape):
+                    raise ValueError(f"an output of {tuple(o.shape)} {o.dtype} for a gradient of {tuple(g.shape)} {g.dtype}")
     if error_if_nonfinite:
         total = grad_norm(grads, norm_type=norm_type)
         if not math.isfinite(float(total)):

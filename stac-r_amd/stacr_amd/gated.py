@@ -52,17 +52,15 @@ class GatedFeedForwardFunction(torch.autograd.Function):
         x2d = x if x.dim() == 2 else x.reshape(-1, x.shape[-1])
         h = kernels.gated_forward(x2d, w_gate, w_up, _contiguous(b_gate), _contiguous(b_up), activation,
                                   None if recompute else "full")
-        kept = (None,) * 4
-        if not recompute:
-            h, kept = h
-        ctx.save_for_backward(x, w_gate, w_up, b_gate, b_up, *kept)
+        h, kept = (h, None) if recompute else h
+        ctx.save_for_backward(x, w_gate, w_up, b_gate, b_up, kept)
         ctx.activation = activation
         return h if x.dim() == 2 else h.view(*x.shape[:-1], h.shape[1])
 
     @staticmethod
     @once_differentiable
     def backward(ctx, dh):
-        x, w_gate, w_up, b_gate, b_up, *kept = ctx.saved_tensors
+        x, w_gate, w_up, b_gate, b_up, kept = ctx.saved_tensors
         need = ctx.needs_input_grad
         if x.dim() != 2:
             dh, x2d = dh.reshape(-1, dh.shape[-1]), x.reshape(-1, x.shape[-1])
@@ -70,7 +68,7 @@ class GatedFeedForwardFunction(torch.autograd.Function):
             x2d = x
         dx, dwg, dwu, dbg, dbu, _ = kernels.gated_backward(
             dh, x2d, w_gate, w_up, _contiguous(b_gate), _contiguous(b_up), ctx.activation,
-            None if kept[0] is None else kept, (need[0], need[1] or need[2], need[3], need[4]))
+            kept, (need[0], need[1] or need[2], need[3], need[4]))
         if dx is not None and x.dim() != 2:
             dx = dx.view(x.shape)
         return dx, dwg if need[1] else None, dwu if need[2] else None, dbg, dbu, None, None
@@ -121,7 +119,7 @@ class STACRGatedFunction(torch.autograd.Function):
             mode, budget = "chunk_topk", 0.0
         coeff, idx, data, scale, census, bits, _ = _save_factors(x2d, basis.to(x.dtype), mode, float(budget), int(bits),
                                                                  int(chunk_rows), int(block_size), float(sample_ratio))
-        ctx.save_for_backward(w_gate, w_up, b_gate, b_up, coeff, basis.to(x.dtype), idx, data, scale, kept[0], kept[1])
+        ctx.save_for_backward(w_gate, w_up, b_gate, b_up, coeff, basis.to(x.dtype), idx, data, scale, kept)
         # the save's entry census (an intermediate, outside the saved tensors): the weight gradient need not count
         ctx.census = census if idx is not None else None
         ctx.bits, ctx.shape, ctx.activation = bits if idx is not None else 0, x.shape, activation
@@ -130,13 +128,13 @@ class STACRGatedFunction(torch.autograd.Function):
     @staticmethod
     @once_differentiable
     def backward(ctx, dh):
-        w_gate, w_up, b_gate, b_up, coeff, q, idx, data, scale, gate, up = ctx.saved_tensors
+        w_gate, w_up, b_gate, b_up, coeff, q, idx, data, scale, kept = ctx.saved_tensors
         need = ctx.needs_input_grad
         weights = need[1] or need[2]
         with torch.autocast(device_type=dh.device.type, enabled=False):
             dx, _, _, dbg, dbu, dgu = kernels.gated_backward(
                 dh.reshape(-1, dh.shape[-1]), None, w_gate, w_up, _contiguous(b_gate), _contiguous(b_up), ctx.activation,
-                (gate, up, None, None), (need[0], False, need[3], need[4]), slopes=weights)
+                kept, (need[0], False, need[3], need[4]), slopes=weights)
             dwg = dwu = None
             if weights:
                 residual = (idx, data, scale) if idx is not None and idx.numel() else None
@@ -197,7 +195,8 @@ class STACRGatedFeedForward(nn.Module):
     def stored_bytes(self, rows: int, value_bytes: int = 2) -> dict:
         """STACRLinear.stored_bytes of the shared input, and the kept pre-activations."""
         stored = self.gate.stored_bytes(rows, value_bytes)
-        stored["preactivations"] = 2 * int(rows) * ((self.out_features + 7) // 8 * 8) * value_bytes
+        each = int(rows) * ((self.out_features + 7) // 8 * 8) * value_bytes
+        stored["preactivations"] = 2 * ((each + 255) // 256 * 256)
         stored["total"] += stored["preactivations"]
         return stored
 

@@ -607,28 +607,50 @@ def _rows_of(x2d):
 def gated_forward(x2d: torch.Tensor, w_gate: torch.Tensor, w_up: torch.Tensor, b_gate: torch.Tensor | None = None,
                   b_up: torch.Tensor | None = None, activation: str = "silu", keep: str | None = None):
     """h = act(x Wg^T + bg) * (x Wu^T + bu) of rows x d (stacr_gated_forward).  ``keep`` "type" or "full": also
-    the pre-activations for gated_backward, (h, kept): rounded to the type, or 16-bit types in 24 bits.  The
-    caller has checked shapes, types and devices (gated.gated_feed_forward does)."""
+    the pre-activations for gated_backward, (h, kept) with one buffer of bytes: rounded to the type, or 16-bit
+    types in 24 bits.  The caller has checked shapes, types and devices (gated.gated_feed_forward does)."""
     x2d, x_ld = _rows_of(x2d)
     w_gate, w_up = w_gate.contiguous(), w_up.contiguous()
     rows, d = x2d.shape
     ff = w_gate.shape[0]
     code = dtype_code(x2d.dtype)
     h = x2d.new_empty((rows, ff))
-    gate = up = gate_low = up_low = None
+    kept, at = None, (None,) * 4
     if keep is not None:
-        shape = (rows, (ff + 7) // 8 * 8)  # rows padded to whole pieces of 8
-        gate, up = h.new_empty(shape), h.new_empty(shape)
-        if keep == "full" and code != _lib.DTYPE_F32:
-            gate_low, up_low = h.new_empty(shape, dtype=torch.uint8), h.new_empty(shape, dtype=torch.uint8)
-    ws, nbytes = (None, 0) if rows <= GATED_FEW_ROWS else _gated_workspace(x2d, code, rows, d, x_ld, w_gate, w_up, 0)
+        kept = h.new_empty(_kept_bytes(rows, ff, code, keep == "full"), dtype=torch.uint8)
+        at = _kept_parts(kept, rows, ff, code)
+    # nothing to lay out anew: aligned rows of whole pieces in a 16-bit type
+    plain = rows <= GATED_FEW_ROWS or (code and not (d | x_ld) & 7 and
+                                       not (x2d.data_ptr() | w_gate.data_ptr() | w_up.data_ptr()) & 15)
+    ws, nbytes = (None, 0) if plain else _gated_workspace(x2d, code, rows, d, x_ld, w_gate, w_up, 0)
     rc = _lib.load().stacr_gated_forward(x2d.data_ptr(), code, rows, d, x_ld, w_gate.data_ptr(), w_up.data_ptr(), ff,
                                          _at(b_gate), _at(b_up), _lib.ACTIVATION_CODES[activation], h.data_ptr(),
-                                         _at(gate), _at(up), _at(gate_low), _at(up_low), _at(ws), nbytes,
-                                         _raw_stream(x2d))
+                                         at[0], at[1], at[2], at[3], _at(ws), nbytes, _raw_stream(x2d))
     if rc:
         _lib.check(rc, "stacr_gated_forward")
-    return h if keep is None else (h, (gate, up, gate_low, up_low))
+    return h if keep is None else (h, kept)
+
+
+def _kept_bytes(rows, ff, code, full):
+    """Bytes of the kept pre-activations: rows of ff rounded up to 8 values of g and of u in the type, and in
+    full for the 16-bit types their low bytes after them; each of the four on its own 256-byte line."""
+    n = rows * ((ff + 7) // 8 * 8)
+    size = 2 if code else 4
+    return 2 * _lines(n * size) + (2 * _lines(n) if full and code else 0)
+
+
+def _lines(n):
+    return (n + 255) // 256 * 256
+
+
+def _kept_parts(kept, rows, ff, code):
+    """Addresses of g, u and their low bytes (None where not kept) in a buffer of _kept_bytes."""
+    n = rows * ((ff + 7) // 8 * 8)
+    whole = _lines(n * (2 if code else 4))
+    at = kept.data_ptr()
+    if not code or kept.numel() == 2 * whole:
+        return at, at + whole, None, None
+    return at, at + whole, at + 2 * whole, at + 2 * whole + _lines(n)
 
 
 def gated_backward(dh: torch.Tensor, x2d: torch.Tensor | None, w_gate: torch.Tensor, w_up: torch.Tensor,
@@ -648,12 +670,12 @@ def gated_backward(dh: torch.Tensor, x2d: torch.Tensor | None, w_gate: torch.Ten
     dbg = dh.new_empty(ff) if needs[2] else None
     dbu = dh.new_empty(ff) if needs[3] else None
     dgu = dh.new_empty((rows, 2 * ((ff + 7) // 8 * 8))) if slopes else None
-    gate, up, gate_low, up_low = kept if kept is not None else (None,) * 4
+    at = _kept_parts(kept, rows, ff, code) if kept is not None else (None,) * 4
     ws, nbytes = _gated_workspace(x2d, code, rows, d, x_ld, w_gate, w_up, 1)
     rc = _lib.load().stacr_gated_backward(dh.data_ptr(), _at(x2d), code, rows, d, x_ld, w_gate.data_ptr(),
                                           w_up.data_ptr(), ff, _at(b_gate), _at(b_up),
-                                          _lib.ACTIVATION_CODES[activation], _at(gate), _at(up), _at(gate_low),
-                                          _at(up_low), _at(dx), _at(dwg), _at(dwu), _at(dbg), _at(dbu), _at(dgu),
+                                          _lib.ACTIVATION_CODES[activation], at[0], at[1], at[2], at[3],
+                                          _at(dx), _at(dwg), _at(dwu), _at(dbg), _at(dbu), _at(dgu),
                                           _at(ws), nbytes, _raw_stream(dh))
     if rc:
         _lib.check(rc, "stacr_gated_backward")

@@ -280,7 +280,8 @@ def test_kept_preactivations(dev, rows, d, ff, dtype):
     announce("gated kept", rows, d, ff, dtype)
     (x, wg, wu, bg, bu), dh = make(rows, d, ff, dtype, dev)
     h, kept = kernels.gated_forward(x, wg, wu, bg, bu, "silu", keep="type")
-    g = kept[0]
+    pad = (ff + 7) // 8 * 8
+    g = kept[:rows * pad * h.element_size()].view(h.dtype).view(rows, pad)
     assert torch.equal(h, kernels.gated_forward(x, wg, wu, bg, bu, "silu"))
     g64 = x.double() @ wg.double().t() + bg.double()
     assert off(g[:, :ff], g64) <= tolerance(dtype, d, False)
@@ -291,7 +292,6 @@ def test_kept_preactivations(dev, rows, d, ff, dtype):
     room = 1.5 if half else 1.0
     for a, b in zip((dx, dwg, dwu, dbg, dbu), want):
         assert off(a, b) <= room * tolerance(dtype, max(rows, d, ff), True)
-    pad = (ff + 7) // 8 * 8
     assert dgu.shape == (rows, 2 * pad) and not dgu[:, ff:pad].any() and not dgu[:, pad + ff:].any()
     assert off(dgu[:, :ff].double().t() @ x.double(), want[1]) <= room * tolerance(dtype, max(rows, d, ff), True)
     alone = kernels.gated_backward(dh, None, wg, wu, bg, bu, "silu", kept=kept, needs=(True, False, False, False),
@@ -320,3 +320,48 @@ def test_refusals(dev):
         f(x, wg, wu.cpu())
     with pytest.raises(TypeError, match="float32, bfloat16 and float16"):
         f(x.double(), wg.double(), wu.double())
+
+
+def test_in_a_graph(dev):
+    """Both passes captured once and replayed on other inputs, eager work between."""
+    from stacr_amd import kernels
+
+    announce("gated graph")
+    for dtype in ("bf16", "f32"):
+        (x, wg, wu, _, _), dh = make(200, 136, 72, dtype, dev)
+
+        def both():
+            h, kept = kernels.gated_forward(x, wg, wu, keep="full")
+            return (h, *kernels.gated_backward(dh, x, wg, wu, kept=kept)[:3])
+
+        s = torch.cuda.Stream()
+        with torch.cuda.stream(s):
+            both()
+        s.synchronize()
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            out = both()
+        for _ in range(3):
+            x.normal_()
+            dh.normal_()
+            graph.replay()
+            torch.cuda.synchronize()
+            for a, b in zip(out, both()):
+                assert torch.equal(a, b)
+
+
+def test_large_gates_have_finite_slopes(dev):
+    """Gates whose squares fp32 cannot hold: the slope's tail is 0 or 1, not infinity times 0."""
+    import stacr_amd
+
+    announce("gated large gates")
+    x = torch.full((3, 8), 3.0e19, device=dev)
+    x[1] = -3.0e19
+    w, one = torch.eye(8, device=dev), torch.zeros(8, 8, device=dev)
+    for act in ACTS:
+        leaf = x.clone().requires_grad_(True)
+        h = stacr_amd.gated_feed_forward(leaf, w, one, None, torch.ones(8, device=dev), activation=act)
+        dx, = torch.autograd.grad(h, leaf, torch.ones_like(h))
+        want = 0.0 if act == "sigmoid" else 1.0
+        assert torch.equal(dx[0], torch.full((8,), want, device=dev)), act
+        assert not dx[1].any(), act
