@@ -18,16 +18,20 @@ ACTIVATIONS = tuple(_lib.ACTIVATION_CODES)
 
 
 def _check_gated(x, w_gate, w_up, b_gate, b_up, activation) -> None:
+    # the usual case in few steps: a call on a single token is bound by the host
+    dtype, index, shape = x.dtype, x.get_device(), w_gate.shape
+    if (b_gate is None and b_up is None and index >= 0 and activation in _lib.ACTIVATION_CODES and len(shape) == 2 and
+            shape == w_up.shape and shape[0] and x.shape[-1:] == shape[1:] and w_gate.dtype is dtype and
+            w_up.dtype is dtype and w_gate.get_device() == index and w_up.get_device() == index and shape[1]):
+        return
     if activation not in _lib.ACTIVATION_CODES:
         raise ValueError(f"activation must be one of {list(ACTIVATIONS)}, got {activation!r}")
     kernels.require_gpu(x, "input")
-    shape = w_gate.shape
     if len(shape) != 2 or shape != w_up.shape or 0 in shape:
         raise ValueError(f"w_gate and w_up must be two (ff, d) matrices of one shape, got {tuple(shape)} and "
                          f"{tuple(w_up.shape)}")
-    if x.dim() < 1 or x.shape[-1] != shape[1]:
+    if x.shape[-1:] != shape[1:]:
         raise ValueError(f"Expected last input dimension {shape[1]}, got {tuple(x.shape)}")
-    dtype, index = x.dtype, x.get_device()
     for name, t in (("w_gate", w_gate), ("w_up", w_up), ("b_gate", b_gate), ("b_up", b_up)):
         if t is None:
             continue
@@ -88,8 +92,8 @@ def gated_feed_forward(x: torch.Tensor, w_gate: torch.Tensor, w_up: torch.Tensor
     16-bit training keeps of this block (g, act(g) and u).  ``recompute=True`` keeps nothing but the input
     and forms them again in the backward: the same gradients up to the 24 bits' rounding, at a third more work.
     """
-    if torch.is_autocast_enabled(x.device.type):
-        dtype = torch.get_autocast_dtype(x.device.type)
+    if torch.is_autocast_enabled("cuda"):
+        dtype = torch.get_autocast_dtype("cuda")
         x, w_gate, w_up, b_gate, b_up = (None if t is None else t.to(dtype) for t in (x, w_gate, w_up, b_gate, b_up))
     _check_gated(x, w_gate, w_up, b_gate, b_up, activation)
     if torch.is_grad_enabled() and (x.requires_grad or w_gate.requires_grad or w_up.requires_grad or
@@ -183,8 +187,8 @@ class STACRGatedFeedForward(nn.Module):
         if not (self.training and torch.is_grad_enabled() and x.numel() > 0 and
                 (gate.weight.requires_grad or self.up_weight.requires_grad)):
             return gated_feed_forward(x, *w, activation=self.activation)
-        if torch.is_autocast_enabled(x.device.type):
-            dtype = torch.get_autocast_dtype(x.device.type)
+        if torch.is_autocast_enabled("cuda"):
+            dtype = torch.get_autocast_dtype("cuda")
             x, *w = (None if t is None else t.to(dtype) for t in (x, *w))
         _check_gated(x, *w, self.activation)
         basis, budget = gate._factor_state(x)

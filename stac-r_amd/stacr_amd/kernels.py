@@ -615,6 +615,14 @@ def gated_forward(x2d: torch.Tensor, w_gate: torch.Tensor, w_up: torch.Tensor, b
     ff = w_gate.shape[0]
     code = dtype_code(x2d.dtype)
     h = x2d.new_empty((rows, ff))
+    lib = _lib.load()
+    if rows <= GATED_FEW_ROWS and keep is None:  # no workspace, nothing kept: the least a call can be
+        rc = lib.stacr_gated_forward(x2d.data_ptr(), code, rows, d, x_ld, w_gate.data_ptr(), w_up.data_ptr(), ff,
+                                     _at(b_gate), _at(b_up), _lib.ACTIVATION_CODES[activation], h.data_ptr(), None, None,
+                                     None, None, None, 0, _raw_stream(x2d))
+        if rc:
+            _lib.check(rc, "stacr_gated_forward")
+        return h
     kept, at = None, (None,) * 4
     if keep is not None:
         kept = h.new_empty(_kept_bytes(rows, ff, code, keep == "full"), dtype=torch.uint8)
@@ -623,9 +631,9 @@ def gated_forward(x2d: torch.Tensor, w_gate: torch.Tensor, w_up: torch.Tensor, b
     plain = rows <= GATED_FEW_ROWS or (code and not (d | x_ld) & 7 and
                                        not (x2d.data_ptr() | w_gate.data_ptr() | w_up.data_ptr()) & 15)
     ws, nbytes = (None, 0) if plain else _gated_workspace(x2d, code, rows, d, x_ld, w_gate, w_up, 0)
-    rc = _lib.load().stacr_gated_forward(x2d.data_ptr(), code, rows, d, x_ld, w_gate.data_ptr(), w_up.data_ptr(), ff,
-                                         _at(b_gate), _at(b_up), _lib.ACTIVATION_CODES[activation], h.data_ptr(),
-                                         at[0], at[1], at[2], at[3], _at(ws), nbytes, _raw_stream(x2d))
+    rc = lib.stacr_gated_forward(x2d.data_ptr(), code, rows, d, x_ld, w_gate.data_ptr(), w_up.data_ptr(), ff,
+                                 _at(b_gate), _at(b_up), _lib.ACTIVATION_CODES[activation], h.data_ptr(), *at, _at(ws),
+                                 nbytes, _raw_stream(x2d))
     if rc:
         _lib.check(rc, "stacr_gated_forward")
     return h if keep is None else (h, kept)

@@ -41,30 +41,38 @@ def rotary_tables(length: int, rot: int, *, base: float = 10000.0, scaling: str 
 
 
 def _check_rotary(q, k, cos, sin, positions, layout) -> None:
+    # the usual case in few steps: a call on single tokens is bound by the host
+    shape, dtype, index, table = q.shape, q.dtype, q.get_device(), cos.shape
+    if (len(shape) == 4 and index >= 0 and layout in _lib.ROTARY_LAYOUTS and dtype in kernels.DTYPE_CODES and
+            k is not None and k.dtype is dtype and k.dim() == 4 and k.get_device() == index and
+            k.shape[:2] == shape[:2] and k.shape[3] == shape[3] and len(table) == 2 and table == sin.shape and
+            cos.dtype is torch.float32 and sin.dtype is torch.float32 and 2 <= 2 * table[1] <= shape[3] and
+            cos.get_device() == index and sin.get_device() == index and positions is not None and
+            positions.dtype is torch.int64 and positions.shape == shape[:2] and positions.get_device() == index):
+        return
     if layout not in _lib.ROTARY_LAYOUTS:
         raise ValueError(f"layout must be one of {list(_lib.ROTARY_LAYOUTS)}, got {layout!r}")
     kernels.require_gpu(q, "queries")
-    kernels.dtype_code(q.dtype)
-    if q.dim() != 4:
+    kernels.dtype_code(dtype)
+    if len(shape) != 4:
         raise ValueError(f"queries are batch x seq x heads x head, got {q.dim()} dimensions")
     if k is not None:
-        if k.dim() != 4 or k.shape[:2] != q.shape[:2] or k.shape[3] != q.shape[3]:
-            raise ValueError(f"keys {tuple(k.shape)} do not match queries {tuple(q.shape)}")
-        if k.dtype != q.dtype:
-            raise TypeError(f"keys are {k.dtype}, queries {q.dtype}")
-    if cos.dim() != 2 or cos.shape != sin.shape:
-        raise ValueError(f"cos and sin must be two (positions, rot / 2) tables, got {tuple(cos.shape)} and "
+        if k.dim() != 4 or k.shape[:2] != shape[:2] or k.shape[3] != shape[3]:
+            raise ValueError(f"keys {tuple(k.shape)} do not match queries {tuple(shape)}")
+        if k.dtype != dtype:
+            raise TypeError(f"keys are {k.dtype}, queries {dtype}")
+    if len(table) != 2 or table != sin.shape:
+        raise ValueError(f"cos and sin must be two (positions, rot / 2) tables, got {tuple(table)} and "
                          f"{tuple(sin.shape)}")
     if cos.dtype != torch.float32 or sin.dtype != torch.float32:
         raise TypeError("cos and sin must be float32")
-    if not 2 <= 2 * cos.shape[1] <= q.shape[3]:
-        raise ValueError(f"tables of {cos.shape[1]} pairs do not fit heads of {q.shape[3]} features")
+    if not 2 <= 2 * table[1] <= shape[3]:
+        raise ValueError(f"tables of {table[1]} pairs do not fit heads of {shape[3]} features")
     if positions is not None:
         if positions.dtype not in (torch.int32, torch.int64):
             raise TypeError(f"positions must be int32 or int64, got {positions.dtype}")
-        if positions.shape not in ((q.shape[1],), (q.shape[0], q.shape[1])):
+        if positions.shape not in (shape[1:2], shape[:2]):
             raise ValueError(f"positions must be (seq,) or (batch, seq), got {tuple(positions.shape)}")
-    index = q.get_device()
     for t in (k, cos, sin, positions):
         if t is not None and t.get_device() != index:
             raise RuntimeError(f"rotary: tensors on {t.device} and {q.device}")
