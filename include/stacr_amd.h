@@ -34,6 +34,8 @@
  *   stacr_c1_*               the C1 checkpoint-boundary codec's device work,
  *                            CheckpointBoundaryCodec.pack_tensor / unpack_record,
  *                            stacr/protocols/checkpointing.py:374-400,411-545
+ * Without a counterpart there: stacr_gated_*, stacr_rotary*, stacr_clip_* (what a training step runs
+ * between the compressed projections).
  */
 #ifndef STACR_AMD_H
 #define STACR_AMD_H
