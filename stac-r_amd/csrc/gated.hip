@@ -3,8 +3,8 @@
 //   forward    one product over [Wg; Wu] whose tiles hold a gate column block beside the same up
 //              columns, so that a lane ends with both pre-activations of its outputs and the epilogue
 //              writes h = act(g) u alone
-//   backward   dg = dh u act'(g), du = dh act(g): the same product again with another epilogue (nothing
-//              but x is kept by the forward), or an elementwise pass where g and u were kept; then
+//   backward   dg = dh u act'(g), du = dh act(g): an elementwise pass over g and u, which the forward
+//              kept, or, where it kept x alone, the same product again with another epilogue; then
 //              dx = dg Wg + du Wu (one product, K over both halves), [dWg; dWu] = [dg | du]^T x
 //   few rows   a workgroup of four waves takes 16 outputs of both projections, each wave a quarter of
 //              K: the weights are read once, straight into the operands
@@ -179,6 +179,13 @@ template <typename T> __device__ __forceinline__ uint4 get8(const T *p, int64_t 
 template <int DT> __device__ __forceinline__ uint2 pack4(const float (&v)[4])
 {
     using A = Act<DT>;
+    if constexpr (DT == STACR_DTYPE_BF16) {  // one instruction a pair
+        typedef float F2 __attribute__((ext_vector_type(2)));
+        typedef __bf16 B2 __attribute__((ext_vector_type(2)));
+        const F2 x = {v[0], v[1]}, y = {v[2], v[3]};
+        return make_uint2(__builtin_bit_cast(uint32_t, __builtin_convertvector(x, B2)),
+                          __builtin_bit_cast(uint32_t, __builtin_convertvector(y, B2)));
+    }
     return make_uint2((uint32_t)A::st(v[0]) | (uint32_t)A::st(v[1]) << 16, (uint32_t)A::st(v[2]) | (uint32_t)A::st(v[3]) << 16);
 }
 
@@ -226,36 +233,65 @@ __device__ __forceinline__ void put_slopes(uint16_t *p, int64_t plane, int lane,
     }
 }
 
-// the kept pre-activations of the same: in the type, or the upper 16 of 24 bits and the low byte
-template <int DT>
-__device__ __forceinline__ void put_kept(void *p, uint8_t *low, int64_t at, int lane, const float (&a)[4], const float (&b)[4],
-                                         int64_t n, int64_t N, bool in)
-{
-    if (DT == STACR_DTYPE_F32 || !low) {
-        put_blocks<DT>(static_cast<typename Act<DT>::T *>(p) + at, lane, a, b, n, N, in);
-        return;
+// A wave's rows, from its first on, of a result whose rows are multiples of 16 bytes: stores without a branch,
+// as the buffer's range drops the rows past the last and a column past the last gets an offset past the range.
+// For the forward's 8 bytes an output (32768 x 2048 x 8192: 2164 -> 2094 us against stores that each test their
+// place; a plain product, with a quarter of that to write, gains nothing by it).
+struct EvenRows {
+    __amdgpu_buffer_rsrc_t r;
+    uint32_t row;  // bytes of a row
+
+    __device__ __forceinline__ EvenRows(void *p, int64_t first, int64_t rows, int64_t bytes)
+        : r(mm_rsrc(static_cast<unsigned char *>(p) + first * bytes, (rows - first) * bytes)), row((uint32_t)bytes)
+    {
     }
+    // this lane's place in the wave's first 16 rows
+    __device__ __forceinline__ uint32_t at(int lane, int64_t n, int64_t N, int size) const
+    {
+        return (lane & 15) * row + (n < N ? (uint32_t)n * size : kMmPast);
+    }
+    __device__ __forceinline__ void put(uint32_t at, uint4 v) const
+    {
+        typedef uint32_t U4 __attribute__((ext_vector_type(4)));
+        __builtin_amdgcn_raw_buffer_store_b128(U4{v.x, v.y, v.z, v.w}, r, at, 0, 0);
+    }
+    __device__ __forceinline__ void put(uint32_t at, uint2 v) const
+    {
+        typedef uint32_t U2 __attribute__((ext_vector_type(2)));
+        __builtin_amdgcn_raw_buffer_store_b64(U2{v.x, v.y}, r, at, 0, 0);
+    }
+};
+
+// As put_blocks, for the wave's rows 16 i + lane % 16
+template <int DT>
+__device__ __forceinline__ void put_even(const EvenRows &rows, int i, int lane, const float (&a)[4], const float (&b)[4],
+                                         int64_t n, int64_t N)
+{
+    const uint4 v = eights(pack4<DT>(a), pack4<DT>(b));
+    rows.put(rows.at(lane, n + (lane >> 4) * 8, N, 2) + i * 16 * rows.row, v);
+}
+
+// rows of N 16-bit values, `ld` apart, that are eights of them at multiples of 16 bytes
+__device__ __forceinline__ bool even_rows(const void *p, int64_t N, int64_t ld)
+{
+    return ((N | ld) & 7) == 0 && (reinterpret_cast<uintptr_t>(p) & 15) == 0;
+}
+
+// Upper 16 of the 24 bits of two quads of neighbouring blocks, as eights, and the lower 8 of them
+__device__ __forceinline__ void to_kept(const float (&a)[4], const float (&b)[4], uint4 &high, uint2 &low)
+{
     uint32_t x[4], y[4];
 #pragma unroll
     for (int r = 0; r < 4; ++r) x[r] = to_24(a[r]), y[r] = to_24(b[r]);
-    const uint4 v = eights(make_uint2(x[0] >> 16 | (x[1] & 0xffff0000u), x[2] >> 16 | (x[3] & 0xffff0000u)),
-                           make_uint2(y[0] >> 16 | (y[1] & 0xffff0000u), y[2] >> 16 | (y[3] & 0xffff0000u)));
-    uint32_t lx = 0, ly = 0;
-#pragma unroll
-    for (int r = 0; r < 4; ++r) lx |= (x[r] >> 8 & 255u) << r * 8, ly |= (y[r] >> 8 & 255u) << r * 8;
-    mm_eights(lx, ly);
-    if (!in) return;
-    n += (lane >> 4) * 8;
-    put8(static_cast<uint16_t *>(p) + at, v, n, N);
-    uint8_t *q = low + at + n;
-    if (n + 8 <= N) {
-        const uint2 w = make_uint2(lx, ly);
-        __builtin_memcpy(q, &w, 8);
-    } else {
-#pragma unroll
-        for (int k = 0; k < 8; ++k)
-            if (n + k < N) q[k] = (uint8_t)((k < 4 ? lx : ly) >> (k & 3) * 8);
-    }
+    // (bytes of __builtin_amdgcn_perm's result: 0 to 3 name the second operand's, 4 to 7 the first's)
+    const auto upper = [](uint32_t p, uint32_t q) { return __builtin_amdgcn_perm(q, p, 0x07060302u); };
+    const auto lower = [](const uint32_t (&v)[4]) {
+        const uint32_t p = __builtin_amdgcn_perm(v[1], v[0], 0x0c0c0501u), q = __builtin_amdgcn_perm(v[3], v[2], 0x05010c0cu);
+        return p | q;
+    };
+    high = eights(make_uint2(upper(x[0], x[1]), upper(x[2], x[3])), make_uint2(upper(y[0], y[1]), upper(y[2], y[3])));
+    low = make_uint2(lower(x), lower(y));
+    mm_eights(low.x, low.y);
 }
 
 // A workgroup takes every gridDim.x-th tile.  Consecutive logical tiles share an XCD (workgroups are dealt
@@ -467,6 +503,8 @@ __global__ __launch_bounds__(WM *WN * 64, 1) void k_gated_mm(const MmArgs p)
                     }
             }
             if constexpr (EPI == kFwd) {
+                const bool even = even_rows(p.out, p.N, p.ldo);
+                const EvenRows rows(p.out, t.m0 + wm * TM, p.M, p.ldo * 2);
                 with_activation(p.act, [&](auto c) __attribute__((always_inline)) {
 #pragma unroll
                     for (int i = 0; i < MI; ++i) {
@@ -482,24 +520,47 @@ __global__ __launch_bounds__(WM *WN * 64, 1) void k_gated_mm(const MmArgs p)
                                     activate<EXACT, decltype(c)::value>(acc[i][j + 2 * b][r], a, slope);
                                     h[b][r] = a * acc[i][j + 2 * b + 1][r];
                                 }
+                            if constexpr (!EXACT) {
+                                if (even) {
+                                    put_even<DT>(rows, i, lane, h[0], h[1], f0 + j * 8, p.N);
+                                    continue;
+                                }
+                            }
                             put_blocks<DT>(static_cast<T *>(p.out) + m * p.ldo, lane, h[0], h[1], f0 + j * 8, p.N, m < p.M);
                         }
                     }
                 });
-                if (p.gate) {
+                if (p.gate) {  // rows of ff_pad values, a multiple of 8
+                    const int64_t first = t.m0 + wm * TM;
 #pragma unroll
-                    for (int i = 0; i < MI; ++i) {
-                        const int64_t m = mfirst + i * 16;
+                    for (int u = 0; u < 2; ++u) {
+                        void *o = u ? p.up : p.gate;
+                        const EvenRows k(o, first, p.M, p.ff_pad * 2);
+                        const EvenRows l(u ? p.up_low : p.gate_low, first, p.gate_low ? p.M : first, p.ff_pad);
 #pragma unroll
-                        for (int j = 0; j < NI; j += 4)
+                        for (int j = 0; j < NI; j += 4) {
+                            const int64_t f = f0 + j * 8;
+                            const uint32_t at = k.at(lane, f + (lane >> 4) * 8, p.ff_pad, 2);
+                            const uint32_t low = l.at(lane, f + (lane >> 4) * 8, p.ff_pad, 1);
 #pragma unroll
-                            for (int u = 0; u < 2; ++u) {
+                            for (int i = 0; i < MI; ++i) {
                                 float a[4], b[4];
                                 quad(acc[i][j + u], a);
                                 quad(acc[i][j + 2 + u], b);
-                                put_kept<DT>(u ? p.up : p.gate, u ? p.up_low : p.gate_low, m * p.ff_pad, lane, a, b, f0 + j * 8,
-                                             p.ff_pad, m < p.M);
+                                if constexpr (EXACT) {
+                                    const int64_t m = mfirst + i * 16;
+                                    put_blocks<DT>(static_cast<T *>(o) + m * p.ff_pad, lane, a, b, f, p.ff_pad, m < p.M);
+                                } else if (p.gate_low) {
+                                    uint4 v;
+                                    uint2 w;
+                                    to_kept(a, b, v, w);
+                                    k.put(at + i * 16 * k.row, v);
+                                    l.put(low + i * 16 * l.row, w);
+                                } else {
+                                    k.put(at + i * 16 * k.row, eights(pack4<DT>(a), pack4<DT>(b)));
+                                }
                             }
+                        }
                     }
                 }
             } else {
@@ -824,7 +885,8 @@ __global__ __launch_bounds__(kBlock) void k_gated_few(const FewArgs p)
     for (int t = 0; t < NT; ++t) ag[t] = au[t] = mmf4{0.0f, 0.0f, 0.0f, 0.0f};
     // U blocks of 32 of K a wave at a time, their loads all on the way before the first product (a loop over
     // single blocks is not unrolled: matrix instructions do not allow a remainder loop).  One token through
-    // 1024 -> 4096: 7.7 us with one block at a time, 5.4 with eight.
+    // 1024 -> 4096: 7.7 us with one block at a time, 7.0 with eight, by events around the launch (the kernel itself
+    // 4.9 us: 3.4 TB/s of weights that the caches may hold, so its start and its end count as much as the reads).
     constexpr int U = DT == STACR_DTYPE_F32 || !VEC ? 2 : NT == 4 ? 4 : 8;
     const int64_t d = p.d;
     const auto blocks = [&](int64_t k0, auto whole) __attribute__((always_inline)) {
@@ -1028,7 +1090,7 @@ Pieces pieces(const Problem &q, bool backward)
 }
 
 // One element (or piece) a thread.  (4096 workgroups that loop, each time a power of two further on, met in
-// the same memory channels: 268 M slopes took 680 us, 524 without the loop.)
+// the same memory channels: 268 M slopes took 770 us, 617 without the loop.)
 int blocks_for(int64_t n) { return (int)hmin<int64_t>((n + kBlock - 1) / kBlock, 1 << 30); }
 
 template <int DT, int NT> void few_launch(const FewArgs &a, bool vec, hipStream_t s)
