@@ -67,6 +67,25 @@ template <bool EXACT> __device__ __forceinline__ float inverse(float x)
     else return __builtin_amdgcn_rcpf(x);
 }
 
+// The normal distribution below g, bell = exp(-g^2 / 2).  With x = |g| / sqrt(2) the part beyond |g| is
+// erfc(x) / 2 = bell exp(x^2) erfc(x) / 2, and exp(x^2) erfc(x) is smooth and falls like 1 / x: a polynomial
+// without a constant term in t = 1 / (1 + 0.51 x), fitted for the least largest relative error, 9e-7, over
+// 0 <= x <= 10 (in fp32, for g above -4: 2e-6, where 1 + erf(x) in fp32 loses 1e-3).  The library's erf takes
+// about 30 instructions on two paths that a wave mostly takes both.
+__device__ __forceinline__ float normal_below(float g, float bell)
+{
+    const float t = __builtin_amdgcn_rcpf(fmaf(fabsf(g), 0.51f * 0.70710678118654752f, 1.0f));
+    float p = 0.094499744f;
+    p = fmaf(p, t, -0.35913408f);
+    p = fmaf(p, t, 0.35844463f);
+    p = fmaf(p, t, 0.055053536f);
+    p = fmaf(p, t, 0.27906591f);
+    p = fmaf(p, t, 0.28415236f);
+    p = fmaf(p, t, 0.28791749f);
+    const float beyond = 0.5f * p * t * bell;
+    return g < 0.0f ? beyond : 1.0f - beyond;
+}
+
 // act(g) and act'(g)
 template <bool EXACT, int ACT> __device__ __forceinline__ void activate(float g, float &a, float &slope)
 {
@@ -75,9 +94,10 @@ template <bool EXACT, int ACT> __device__ __forceinline__ void activate(float g,
         a = g * s;
         slope = s * (1.0f + g * (1.0f - s));
     } else if constexpr (ACT == STACR_ACT_GELU) {
-        const float below = 0.5f * (1.0f + erff(g * 0.70710678118654752f));
+        const float bell = exp_of<EXACT>(-0.5f * g * g);
+        const float below = EXACT ? 0.5f * (1.0f + erff(g * 0.70710678118654752f)) : normal_below(g, bell);
         a = g * below;
-        slope = below + g * 0.39894228040143268f * exp_of<EXACT>(-0.5f * g * g);
+        slope = below + g * 0.39894228040143268f * bell;
     } else if constexpr (ACT == STACR_ACT_GELU_TANH) {
         const float in = 0.79788456080286536f * (g + 0.044715f * g * g * g);
         const float t = 1.0f - 2.0f * inverse<EXACT>(1.0f + exp_of<EXACT>(2.0f * in));
