@@ -1045,7 +1045,8 @@ int64_t tiles(int64_t m, int64_t n, int bm, int bn) { return ((m + bm - 1) / bm)
 //   256 x 128   8 waves, one workgroup a CU: 0.66 for half the work (LDS and L2 move 1.5 times as much for it)
 //   128 x 128   4 waves, two workgroups a CU: 0.6 for both, half the work together
 // (8192 x 1024 of K 8192, 128 tiles of 256 x 256: 130 us and 20 to join two splits; 256 of 256 x 128: 150 us;
-// 512 of 128 x 128: 130 to 142 us.)
+// 512 of 128 x 128: 130 to 142 us.  Forward, the three in this order: 8192 x 1024 x 4096 187, 211 and 209 us,
+// 3001 x 1000 x 2731 in fp16 83, 79 and 73 us.)
 struct ProductPlan {
     int tile, splits;
 };
